@@ -105,6 +105,12 @@ SIGNATURES = {
     'rag_enc_linear_ln_split_dev': (_i32, [_vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, C.c_float, _i64, _i32, _i32, _vp, _vp, _vp]),
     'rag_enc_linear_ln_split_chain_dev': (_i32, [_vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, C.c_float, _i64, _i32, _i32, _vp, _vp, _vp]),
     'rag_enc_linear_ln_split_pack_dev': (_i32, [_vp, _i32, _i32, _vp, _vp, _vp]),
+    'rag_enc_qk_norm_rope_dev': (_i32, [_vp, _i64, _vp, _vp, _vp, C.c_float, _vp, _i32, _i32, _i64, _i32, _i32, _i32, _i32, _vp, _i64,
+                                        _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp]),
+    'rag_enc_attention_window_workspace': (_i64, [_i64] + [_i32] * 9),
+    'rag_enc_attention_window_dev': (_i32, [_vp, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _i32, _i32,
+                                            _i32, _i32, _i32, C.c_float, _i32, _i32, _i32, _i32, _vp, _i64, _vp, _i64, _vp]),
+    'rag_enc_linear4_dev': (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _i64, _vp]),
     'rag_enc_linear_ln_split_profile': (_i32, [_i32]),
     'rag_enc_linear_ln_split_profile_read': (_i32, [_vp, _vp, _vp, _i32, C.POINTER(_i32)]),
 }
@@ -192,7 +198,8 @@ def _ptr(t, dtype=None):
 FAULT_NAMES = {1: 'dense candidate list overflow', 2: 'merge selection short', 4: 'bm25 tile list overflow',
                8: 'bm25 posting outside its tile', 16: 'bm25 term id beyond the vocabulary',
                32: 'fusion row outside the canon table', 64: 'cross-encoder pair out of range',
-               128: 'segment offsets out of range', 256: 'token, position or type id outside its embedding table'}
+               128: 'segment offsets out of range', 256: 'token, position or type id outside its embedding table',
+               512: 'key/value row outside its array'}
 
 
 def fault_flags(clear=True):
@@ -1235,3 +1242,194 @@ def enc_linear_ln_split_profile_read():
     check(lib().rag_enc_linear_ln_split_profile_read(ms.ctypes.data, rows.ctypes.data, ks.ctypes.data, 1024, C.byref(n)),
           'rag_enc_linear_ln_split_profile_read')
     return ms[:n.value].copy(), rows[:n.value].copy(), ks[:n.value].copy()
+
+
+# ---- encoders with rotary positions, windowed layers, 4-bit weights ---------------------------------
+def _enc_code(dtype):
+    import torch
+    code = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16}.get(dtype)
+    if code is None:
+        raise ValueError(f"the encoder kernels handle float32, bfloat16 and float16, not {dtype}")
+    return code
+
+
+def _same_device(*tensors):
+    """Every tensor given (None: skipped) is on the current GPU, whose stream the kernels are launched on."""
+    import torch
+    here = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != here:
+            raise ValueError(f"rag_hip launches on the current GPU (cuda:{here}); a tensor is on {t.device}")
+
+
+def _heads_view(t, dtype, name):
+    """(pointer, row stride, head stride) of a [rows, heads, head_dim] tensor whose head rows are contiguous."""
+    if t.dim() != 3 or t.dtype != dtype:
+        raise ValueError(f"{name} must be a {dtype} tensor [rows, heads, head_dim]")
+    if t.shape[2] != 1 and t.stride(2) != 1:
+        raise ValueError(f"the dimensions of a head of {name} must be contiguous")
+    return t.data_ptr(), t.stride(0), t.stride(1)
+
+
+def rope_inv_freq(rot_dim, theta=10000.0, device='cuda'):
+    """Angles per position of a rotation over rot_dim dimensions: theta^(-2i / rot_dim), float64 [rot_dim / 2]."""
+    import torch
+    return torch.from_numpy(float(theta) ** (-np.arange(0, int(rot_dim), 2, dtype=np.float64) / int(rot_dim))).to(device)
+
+
+def enc_qk_norm_rope_dev(qkv, pos, inv_freq, n_q_heads, n_kv_heads, gamma_q=None, gamma_k=None, eps=1e-6, interleaved=False,
+                         q_out=None, k_out=None, v_out=None, kv_row=None):
+    """Norm of every query and key head (gamma_q / gamma_k [D] or None: no norm) and rotation by position in one pass
+    (rag_enc_qk_norm_rope_dev): qkv [T, (n_q_heads + 2 n_kv_heads) * D] (rows may be strided), pos int32 [T], inv_freq
+    float64 [R / 2] (rope_inv_freq; pairs (i, i + R/2), or (2i, 2i + 1) with `interleaved`) -> (q [T, n_q_heads, D],
+    k, v).  By default k is a new tensor [T, n_kv_heads, D] and v the value columns of qkv; with k_out and v_out
+    [rows, n_kv_heads, D] (kept keys and values) token t's go to row kv_row[t] (int64 [T], distinct; < 0: nowhere; None:
+    row t) of those."""
+    import torch
+    if qkv.dim() != 2 or not qkv.is_cuda or (qkv.shape[1] > 1 and qkv.stride(1) != 1):
+        raise ValueError("qkv must be a 2-d GPU tensor with contiguous rows")
+    dt, t, heads = qkv.dtype, qkv.shape[0], n_q_heads + 2 * n_kv_heads
+    code = _enc_code(dt)
+    if n_q_heads < 1 or n_kv_heads < 1 or qkv.shape[1] % heads:
+        raise ValueError("a row of qkv must hold n_q_heads + 2 n_kv_heads heads")
+    d = qkv.shape[1] // heads
+    rot = 2 * inv_freq.shape[0] if inv_freq is not None else 0
+    if pos is not None and tuple(pos.shape) != (t,):
+        raise ValueError("pos must have one entry per token")
+    for g in (gamma_q, gamma_k):
+        if g is not None and tuple(g.shape) != (d,):
+            raise ValueError("gamma_q and gamma_k must have one entry per dimension of a head")
+    if (v_out is not None and k_out is None) or (kv_row is not None and k_out is None):
+        raise ValueError("v_out and kv_row need k_out")
+    if kv_row is not None and tuple(kv_row.shape) != (t,):
+        raise ValueError("kv_row must have one entry per token")
+    if q_out is None:
+        q_out = torch.empty((t, n_q_heads, d), dtype=dt, device=qkv.device)
+    elif tuple(q_out.shape) != (t, n_q_heads, d) or (n_q_heads > 1 and q_out.stride(1) != d):
+        raise ValueError("q_out must be [T, n_q_heads, D] with the heads of a row side by side")
+    if k_out is None:
+        k_out = torch.empty((t, n_kv_heads, d), dtype=dt, device=qkv.device)
+    for name, o in (('k_out', k_out), ('v_out', v_out)):
+        if o is not None and (o.dim() != 3 or tuple(o.shape[1:]) != (n_kv_heads, d) or (kv_row is None and o.shape[0] < t)):
+            raise ValueError(f"{name} must be [rows, n_kv_heads, D] with a row for every token")
+    if v_out is not None and v_out.shape[0] != k_out.shape[0]:
+        raise ValueError("k_out and v_out must have the same rows")
+    _same_device(qkv, pos, inv_freq, gamma_q, gamma_k, q_out, k_out, v_out, kv_row)
+    qp, qs, _ = _heads_view(q_out, dt, 'q_out')
+    kp, krs, khs = _heads_view(k_out, dt, 'k_out')
+    vp, vrs, vhs = _heads_view(v_out, dt, 'v_out') if v_out is not None else (None, 0, 0)
+    stride = qkv.stride(0) if t > 1 else qkv.shape[1]
+    check(lib().rag_enc_qk_norm_rope_dev(qkv.data_ptr(), stride, _ptr(pos, torch.int32), _ptr(gamma_q, dt), _ptr(gamma_k, dt), float(eps),
+                                         _ptr(inv_freq, torch.float64), rot, 1 if interleaved else 0, t, n_q_heads, n_kv_heads, d,
+                                         code, qp, qs if t > 1 else n_q_heads * d, kp, krs, khs, vp, vrs, vhs, _ptr(kv_row, torch.int64),
+                                         k_out.shape[0], _stream()), 'rag_enc_qk_norm_rope_dev')
+    if v_out is None:
+        v_out = qkv.unflatten(1, (heads, d))[:, n_q_heads + n_kv_heads:]
+    return q_out, k_out, v_out
+
+
+def enc_attention_window_dev(q, k, v, cu_q, max_q_len, k_start=None, k_len=None, max_k_len=None, window_left=-1, window_right=-1,
+                             n_sinks=0, scale=None, out=None):
+    """Attention with a sliding window and the first n_sinks keys always visible (rag_enc_attention_window_dev).
+    q [Tq, Hq, D], k and v [Tk, Hkv, D] (views of a projection's rows or of kept keys and values; Hq a multiple of
+    Hkv), cu_q int32 [n_seq + 1] the sequences' query rows, max_q_len the longest.  Without k_start the keys of a
+    sequence are its own rows of k and v; with k_start int64 [n_seq] and k_len int32 [n_seq] (max_k_len the longest) they
+    are the rows k_start .. k_start + k_len, and the last query stands at the last of them.  A query at position p sees
+    keys p - window_left .. p + window_right and keys 0 .. n_sinks - 1 up to p + window_right (-1: no limit).
+    Returns out [Tq, Hq * D]; rows of no sequence are left as they were (undefined in a new tensor)."""
+    import torch
+    dt = q.dtype
+    code = _enc_code(dt)
+    if not q.is_cuda or q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+        raise ValueError("q, k and v must be GPU tensors [rows, heads, head_dim]")
+    tq, hq, d = q.shape
+    tk, hkv, _ = k.shape
+    if k.shape != v.shape or k.shape[2] != d or hkv < 1 or hq < 1 or hq % hkv:
+        raise ValueError("k and v must have the same shape, the head size of q, and a divisor of its heads")
+    if (k_start is None) != (k_len is None):
+        raise ValueError("k_start and k_len come together")
+    n_seq = cu_q.shape[0] - 1
+    if n_seq < 0 or cu_q.dim() != 1:
+        raise ValueError("cu_q must have one entry more than there are sequences")
+    if k_start is None:
+        if tk != tq:
+            raise ValueError("without k_start, k and v must have the rows of q")
+        max_k_len = max_q_len
+    elif tuple(k_start.shape) != (n_seq,) or tuple(k_len.shape) != (n_seq,):
+        raise ValueError("k_start and k_len must have one entry per sequence")
+    elif max_k_len is None:
+        raise ValueError("kept keys need max_k_len, the longest of k_len")
+    if out is None:
+        out = torch.empty((tq, hq * d), dtype=dt, device=q.device)
+    elif tuple(out.shape) != (tq, hq * d) or out.dtype != dt or (tq > 0 and out.stride(1) != 1):
+        raise ValueError("out must be [Tq, Hq * D] of q's type with contiguous rows")
+    _same_device(q, k, v, cu_q, k_start, k_len, out)
+    if hq > 1 and q.stride(1) != d:
+        raise ValueError("the heads of a row of q must lie side by side")
+    qp, qs, _ = _heads_view(q, dt, 'q')
+    kp, krs, khs = _heads_view(k, dt, 'k')
+    vp, vrs, vhs = _heads_view(v, dt, 'v')
+    l = lib()
+    sizes = (n_seq, int(max_q_len), int(max_k_len), hq, hkv, d)
+    window = (int(window_left), int(window_right), int(n_sinks))
+    need = l.rag_enc_attention_window_workspace(tq, *sizes, *window)
+    work = torch.empty((need,), dtype=torch.uint8, device=q.device) if need > 0 else None
+    check(l.rag_enc_attention_window_dev(qp, qs if tq > 1 else hq * d, kp, krs, khs, vp, vrs, vhs, _ptr(cu_q, torch.int32), tq,
+                                         _ptr(k_start, torch.int64), _ptr(k_len, torch.int32), tk, *sizes,
+                                         float(d ** -0.5 if scale is None else scale), *window, code, out.data_ptr(),
+                                         out.stride(0) if tq > 1 else hq * d, _ptr(work), max(need, 0), _stream()),
+          'rag_enc_attention_window_dev')
+    return out
+
+
+def quantize4(weight, group=64, dtype=None, symmetric=False):
+    """Weight [N, K] -> the operands of enc_linear4_dev: (codes uint8 [N, K / 2], scales [N, K / group], offsets like
+    scales or None).  Each group of `group` columns keeps its smallest and largest value (offset and offset + 15
+    scales) or, with `symmetric`, the scale of its largest magnitude at code - 8 = -7 .. 7; scales and offsets are rounded to
+    `dtype` (the weight's) first and the codes chosen for the rounded ones.  Runs once per weight, wherever the weight is."""
+    import torch
+    n, k = weight.shape
+    if group not in (32, 64, 128) or k % group:
+        raise ValueError("the group must be 32, 64 or 128 and divide the columns")
+    dtype = weight.dtype if dtype is None else dtype
+    _enc_code(dtype)
+    w = weight.detach().float().reshape(n, k // group, group)
+    if symmetric:
+        scales, offsets = (w.abs().amax(dim=2) / 7).to(dtype), None
+        low = -8 * scales.float()
+    else:
+        offsets = w.amin(dim=2).to(dtype)
+        scales = ((w.amax(dim=2) - offsets.float()) / 15).clamp_min(0).to(dtype)
+        low = offsets.float()
+    step = scales.float()[:, :, None]
+    code = torch.where(step > 0, (w - low[:, :, None]) / torch.where(step > 0, step, torch.ones_like(step)), torch.full_like(w, 8.0 if symmetric else 0.0))
+    code = code.round().clamp(0, 15).to(torch.uint8).reshape(n, k // 2, 2)
+    return (code[:, :, 0] | (code[:, :, 1] << 4)).contiguous(), scales.contiguous(), offsets.contiguous() if offsets is not None else None
+
+
+def enc_linear4_dev(x, codes, scales, offsets=None, bias=None, out=None):
+    """x @ W.T + bias with weights of 4 bits (rag_enc_linear4_dev): x [M, K] bf16, fp16 or fp32 (rows may be strided), codes uint8
+    [N, K / 2] (column 2i in the low half of byte i), scales and offsets [N, K / group] and bias [N] of x's type;
+    W = scales * code + offsets, without offsets scales * (code - 8) (quantize4).  Made for a query's few tokens."""
+    import torch
+    dt = x.dtype
+    code = _enc_code(dt)
+    if x.dim() != 2 or not x.is_cuda or (x.shape[1] > 1 and x.stride(1) != 1):
+        raise ValueError("x must be a 2-d GPU tensor with contiguous rows")
+    m, k = x.shape
+    n = codes.shape[0]
+    if codes.dim() != 2 or codes.shape[1] * 2 != k or scales.dim() != 2 or scales.shape[0] != n or scales.shape[1] < 1 or k % scales.shape[1]:
+        raise ValueError("codes must be [N, K / 2] and scales [N, K / group]")
+    if offsets is not None and offsets.shape != scales.shape:
+        raise ValueError("offsets must have the shape of scales")
+    if bias is not None and tuple(bias.shape) != (n,):
+        raise ValueError("bias must have one entry per row of the weights")
+    if out is None:
+        out = torch.empty((m, n), dtype=dt, device=x.device)
+    elif tuple(out.shape) != (m, n) or out.dtype != dt or (n > 1 and out.stride(1) != 1):
+        raise ValueError("out must be [M, N] of x's type with contiguous rows")
+    _same_device(x, codes, scales, offsets, bias, out)
+    check(lib().rag_enc_linear4_dev(x.data_ptr(), x.stride(0) if m > 1 else k, _ptr(codes, torch.uint8), _ptr(scales, dt), _ptr(offsets, dt),
+                                    _ptr(bias, dt), m, n, k, k // scales.shape[1], code, out.data_ptr(),
+                                    out.stride(0) if m > 1 else n, _stream()), 'rag_enc_linear4_dev')
+    return out

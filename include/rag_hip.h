@@ -78,6 +78,7 @@ int rag_version(void);
 #define RAG_FAULT_CE_PAIR      64u  /* pair packing: query, chunk row or slot out of range    */
 #define RAG_FAULT_SEGMENT     128u  /* segmented top-k: offsets not ascending / out of range   */
 #define RAG_FAULT_TOKEN       256u  /* embedding lookup: token, position or type id out of range */
+#define RAG_FAULT_KV_ROW      512u  /* kept keys/values: row or row range outside the arrays        */
 int rag_fault_flags(uint32_t* out_flags, int32_t clear);
 
 /* ---- dense exact kNN ----------------------------------------------------------
@@ -542,6 +543,61 @@ int rag_enc_embed_layernorm_split_dev(const int32_t* d_ids, const int32_t* d_typ
 int rag_enc_add_layernorm_dev(const void* d_x, const void* d_residual, const void* d_gamma,
                               const void* d_beta, float eps, int64_t rows, int32_t hidden,
                               int32_t dtype, void* d_out, void* stream);
+
+/* ---- pieces of encoders with rotary positions, windowed layers and 4-bit weights -------------------
+ * What the dense encoders for long texts behind SentenceTransformer.encode (reference
+ * src/indexing/embedder.py:65-71) have in place of learned positions and full attention.  The serving forms:
+ * packed documents, and the few or single new tokens of a query behind keys that are kept between calls.   */
+
+/* Norms of queries and keys for each head and the rotation by position in one pass.  qkv: rows of qkv_stride elements,
+ * [n_q_heads + 2 n_kv_heads][head_dim] each (query, key and value heads), one per token.  For every query and key head x
+ *   n = x * gamma / sqrt(mean(x^2) + eps)          (gamma [head_dim], of the rows' type; NULL: n = x, no norm)
+ *   (n_a, n_b) -> (n_a cos t - n_b sin t, n_b cos t + n_a sin t),  t = pos[token] * inv_freq[i] in 64 bits
+ * for the pairs (a, b) = (i, i + rot_dim / 2), or with `interleaved` (2i, 2i + 1), i < rot_dim / 2; dimensions from
+ * rot_dim on are normalised only.  Queries go to q_out (row = token, heads side by side); keys, and where v_out is given
+ * the values as they are, go to row kv_row[token] (NULL: row = token) of arrays of n_kv_rows rows addressed by a row and
+ * a head stride.  kv_row < 0: the token's key and value are not written; a row at or beyond n_kv_rows is not written
+ * and flagged (RAG_FAULT_KV_ROW); no two tokens may name the same row.  fp32 arithmetic, one rounding per element.
+ * dtype bf16, fp16 or fp32; head_dim 32, 64 or 128; rot_dim a multiple of 8 up to head_dim (0: no rotation, pos and inv_freq may be NULL).
+ * Pointers aligned to 4 elements, strides multiples of 4 elements.  q_out, k_out and v_out may be the query, key and
+ * value columns of qkv itself (in place; kv_row NULL), otherwise they must not overlap it.                   */
+int rag_enc_qk_norm_rope_dev(const void* d_qkv, int64_t qkv_stride, const int32_t* d_pos, const void* d_gamma_q,
+                             const void* d_gamma_k, float eps, const double* d_inv_freq, int32_t rot_dim,
+                             int32_t interleaved, int64_t n_tokens, int32_t n_q_heads, int32_t n_kv_heads,
+                             int32_t head_dim, int32_t dtype, void* d_q_out, int64_t q_stride, void* d_k_out,
+                             int64_t k_row_stride, int64_t k_head_stride, void* d_v_out, int64_t v_row_stride,
+                             int64_t v_head_stride, const int64_t* d_kv_row, int64_t n_kv_rows, void* stream);
+/* Attention with a sliding window and a few first tokens that stay visible.  Sequence i has the query rows
+ * [cu_q[i], cu_q[i+1]) of q (rows of q_stride elements, n_q_heads heads side by side) and the key/value rows
+ * k_start[i] .. k_start[i] + k_len[i] of k and v (addressed by a row and a head stride; total_k rows); with k_start and
+ * k_len NULL its keys are the rows of its queries (self-attention of a packed batch).  Its last query stands at its last
+ * key: query j is at position p = k_len - q_len + j and sees key c if
+ *   c - p <= window_right (-1: no limit; 0: causal)  and  (p - c <= window_left (-1: no limit) or c < n_sinks).
+ * out[row] = sum over the seen keys of softmax(scale q.k) v, head h with key/value head h / (n_q_heads / n_kv_heads);
+ * a query that sees no key gets 0.  Keys and values a query does not see do not enter its result, whatever they hold.
+ * Rows of q that belong to no sequence are not read, the same rows of out not written.  A sequence longer than
+ * max_q_len / max_k_len or reaching beyond its arrays is skipped and flagged (RAG_FAULT_SEGMENT, RAG_FAULT_KV_ROW).
+ * dtype bf16, fp16 (matrix cores, fp32 softmax and sums) or fp32; head_dim 32, 64 or 128; pointers and strides multiples
+ * of 16 bytes; out must not overlap q, k or v.  workspace: rag_enc_attention_window_workspace() bytes for the same sizes (0:
+ * may be NULL), 16-byte aligned, used by this call alone until it has run on its stream.                    */
+int64_t rag_enc_attention_window_workspace(int64_t total_q, int32_t n_seq, int32_t max_q_len, int32_t max_k_len,
+                                           int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
+                                           int32_t window_left, int32_t window_right, int32_t n_sinks);
+int rag_enc_attention_window_dev(const void* d_q, int64_t q_stride, const void* d_k, int64_t k_row_stride,
+                                 int64_t k_head_stride, const void* d_v, int64_t v_row_stride, int64_t v_head_stride,
+                                 const int32_t* d_cu_q, int64_t total_q, const int64_t* d_k_start,
+                                 const int32_t* d_k_len, int64_t total_k, int32_t n_seq, int32_t max_q_len,
+                                 int32_t max_k_len, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, float scale,
+                                 int32_t window_left, int32_t window_right, int32_t n_sinks, int32_t dtype, void* d_out,
+                                 int64_t out_stride, void* d_workspace, int64_t workspace_bytes, void* stream);
+/* y[m][n] = sum_k x[m][k] w[n][k] + bias[n] with weights of 4 bits: w[n][k] = scales[n][k / group] * code + offsets[n][k / group],
+ * without offsets (NULL) scales[n][k / group] * (code - 8).  codes [n][k / 2]: column 2i in the low half of byte i of
+ * the row, column 2i + 1 in its high half; scales, offsets [n][k / group], bias [n] (or NULL) of x's type (bf16, fp16 or
+ * fp32).  Made for the few rows of one query (weights are read once per 64 rows of x); any m works.  fp32 sums.
+ * group 32, 64 or 128, k a multiple of it; x, its rows and the codes aligned to 16 bytes; y must not overlap x.   */
+int rag_enc_linear4_dev(const void* d_x, int64_t x_stride, const uint8_t* d_codes, const void* d_scales,
+                        const void* d_offsets, const void* d_bias, int64_t m, int32_t n, int32_t k, int32_t group,
+                        int32_t dtype, void* d_y, int64_t y_stride, void* stream);
 
 #ifdef __cplusplus
 }

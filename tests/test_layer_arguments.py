@@ -1,0 +1,96 @@
+"""CPU: the entry points of rotary, windowed and 4-bit layers check their arguments before any device call."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+
+def _buf(n):
+    a = np.zeros(n + 16, np.uint8)
+    return a, a.ctypes.data + (-a.ctypes.data) % 16
+
+
+def _rope(**kw):
+    import rag_hip
+    keep, p = _buf(4096)
+    a = dict(qkv=p, stride=96, pos=p, gq=None, gk=None, eps=1e-6, inv=p, rot=32, inter=0, t=1, hq=1, hkv=1, d=32, dt=0, q=p, qs=32, k=p, krs=32, khs=32,
+             v=None, vrs=0, vhs=0, row=None, rows=1, stream=None)
+    a.update(kw)
+    return rag_hip.load_library().rag_enc_qk_norm_rope_dev(*a.values()), rag_hip.last_error()
+
+
+@pytest.mark.parametrize('kw,code', [
+    (dict(dt=7), -1), (dict(d=48), -5), (dict(d=256), -5), (dict(t=-1), -1), (dict(hq=0), -1), (dict(hkv=0), -1), (dict(rot=12), -5), (dict(rot=40), -5),
+    (dict(rot=-8), -5), (dict(rows=0), -1), (dict(qkv=None), -1), (dict(q=None), -1), (dict(k=None), -1), (dict(pos=None), -1), (dict(inv=None), -1),
+    (dict(stride=95), -1), (dict(stride=92), -1), (dict(qs=28), -1), (dict(krs=33), -1), (dict(khs=2), -1), (dict(t=1 << 41, rows=1 << 41), -5)])
+def test_rope_arguments(kw, code):
+    rc, text = _rope(**kw)
+    assert rc == code and 'rag_enc_qk_norm_rope' in text
+
+
+def _window(**kw):
+    import rag_hip
+    keep, p = _buf(4096)
+    a = dict(q=p, qs=32, k=p, krs=32, khs=32, v=p, vrs=32, vhs=32, cu=p, tq=1, ks=None, kl=None, tk=1, n=1, mq=1, mk=1, hq=1, hkv=1, d=32, scale=1.0,
+             left=-1, right=-1, sinks=0, dt=1, out=p, os=32, work=None, bytes=0, stream=None)
+    a.update(kw)
+    return rag_hip.load_library().rag_enc_attention_window_dev(*a.values()), rag_hip.last_error()
+
+
+@pytest.mark.parametrize('kw,code', [
+    (dict(dt=3), -1), (dict(d=48), -5), (dict(n=-1), -1), (dict(mq=-1), -1), (dict(tq=-1), -1), (dict(tk=-1), -1), (dict(tq=1 << 31), -5), (dict(mk=1 << 30), -5),
+    (dict(hq=3, hkv=2), -1), (dict(hkv=0), -1), (dict(left=-2), -1), (dict(right=-2), -1), (dict(sinks=-1), -1), (dict(scale=float('inf')), -1),
+    (dict(q=None), -1), (dict(k=None), -1), (dict(out=None), -1), (dict(cu=None), -1), (dict(qs=24), -1), (dict(qs=33), -1), (dict(os=16), -1), (dict(krs=4), -1), (dict(bytes=-1), -1)])
+def test_window_arguments(kw, code):
+    rc, text = _window(**kw)
+    assert rc == code and 'rag_enc_attention_window' in text
+
+
+def test_window_starts_and_lengths_come_together():
+    keep, p = _buf(64)
+    assert _window(ks=p)[0] == -1 and _window(kl=p)[0] == -1
+
+
+def test_nothing_to_do_is_no_error():
+    assert _rope(t=0, rows=0)[0] == 0 and _window(n=0)[0] == 0 and _window(tq=0, mq=0)[0] == 0 and _linear(m=0)[0] == 0
+
+
+def _linear(**kw):
+    import rag_hip
+    keep, p = _buf(4096)
+    a = dict(x=p, xs=64, codes=p, scales=p, off=None, bias=None, m=1, n=8, k=64, group=32, dt=1, y=p, ys=8, stream=None)
+    a.update(kw)
+    return rag_hip.load_library().rag_enc_linear4_dev(*a.values()), rag_hip.last_error()
+
+
+@pytest.mark.parametrize('kw,code', [
+    (dict(dt=9), -1), (dict(m=-1), -1), (dict(n=0), -1), (dict(k=0), -1), (dict(group=16), -5), (dict(group=64, k=96), -5), (dict(k=48), -5), (dict(m=1 << 31), -5),
+    (dict(x=None), -1), (dict(codes=None), -1), (dict(scales=None), -1), (dict(y=None), -1), (dict(xs=65), -1), (dict(m=2, xs=56), -1), (dict(m=2, ys=7), -1)])
+def test_linear4_arguments(kw, code):
+    rc, text = _linear(**kw)
+    assert rc == code and 'rag_enc_linear4' in text
+
+
+@pytest.mark.parametrize('symmetric', [False, True])
+def test_quantize4_on_the_cpu(symmetric):
+    import rag_hip
+    w = torch.randn((9, 128), generator=torch.Generator().manual_seed(1))
+    codes, scales, off = rag_hip.quantize4(w, 32, symmetric=symmetric)
+    c = torch.stack([codes & 15, codes >> 4], dim=2).reshape(9, 128).double()
+    s = scales.double().repeat_interleave(32, dim=1)
+    o = -8 * s if off is None else off.double().repeat_interleave(32, dim=1)
+    # half a step, and the 32-bit roundings of the step and the quotient (16 steps of 2^-23)
+    assert bool(((c * s + o - w.double()).abs() <= s * (0.5 + 64 * 2.0 ** -23)).all())
+    with pytest.raises(ValueError):
+        rag_hip.quantize4(w, 48)
+    with pytest.raises(ValueError):
+        rag_hip.quantize4(w[:, :96], 64)
+    with pytest.raises(ValueError):
+        rag_hip.quantize4(w, 32, dtype=torch.float64)
+
+
+def test_rope_inv_freq():
+    import rag_hip
+    f = rag_hip.rope_inv_freq(8, 10000.0, device='cpu')
+    assert f.dtype == torch.float64 and np.allclose(f.numpy(), [1, 0.1, 0.01, 0.001], rtol=1e-15)
