@@ -4,6 +4,8 @@
 // reading the weights is what the layer costs.  gfx950 only.
 #include "common.h"
 
+#include <algorithm>
+
 namespace {
 
 typedef __bf16 bf16;
@@ -19,6 +21,7 @@ struct Lin4Args {
     void* y;
     int64_t x_stride, y_stride, m;
     int32_t n, k, group;
+    int32_t chunk;                   // 128-column blocks whose scales are in LDS at a time
 };
 
 // The eight codes of a 32-bit word as eight 16-bit floats 16 + code: the code lands in the top mantissa bits of 16.0, so
@@ -28,16 +31,16 @@ template <> struct Code16<bf16> {
     typedef bf16x8 x8;
     static constexpr uint32_t MASK = 0x00780078u, BASE = 0x41804180u, ONES = 0x3f803f80u;
     __device__ static f32x4 mfma(x8 a, x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
-    __device__ static uint4 unpack(uint32_t w) {
-        return make_uint4((w << 3 & MASK) | BASE, (w >> 1 & MASK) | BASE, (w >> 5 & MASK) | BASE, (w >> 9 & MASK) | BASE);
+    __device__ static uint4 unpack(uint32_t w, uint32_t mask, uint32_t base) {
+        return make_uint4((w << 3 & mask) | base, (w >> 1 & mask) | base, (w >> 5 & mask) | base, (w >> 9 & mask) | base);
     }
 };
 template <> struct Code16<f16> {
     typedef f16x8 x8;
     static constexpr uint32_t MASK = 0x03c003c0u, BASE = 0x4c004c00u, ONES = 0x3c003c00u;
     __device__ static f32x4 mfma(x8 a, x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
-    __device__ static uint4 unpack(uint32_t w) {
-        return make_uint4((w << 6 & MASK) | BASE, (w << 2 & MASK) | BASE, (w >> 2 & MASK) | BASE, (w >> 6 & MASK) | BASE);
+    __device__ static uint4 unpack(uint32_t w, uint32_t mask, uint32_t base) {
+        return make_uint4((w << 6 & mask) | base, (w << 2 & mask) | base, (w >> 2 & mask) | base, (w >> 6 & mask) | base);
     }
 };
 
@@ -83,19 +86,43 @@ template <> struct XFrag<float> {
     }
 };
 
-// A workgroup takes 16 rows of the weights and 16 * MT rows of x; its waves take the 128-column blocks of the weights in
-// turn and add their sums up through LDS.  x is the A operand of v_mfma_f32_16x16x32, the codes are the B operand, so a lane
-// ends with its own weight row's sums for four rows of x, and a group's scale is one value per lane.
+// A group's scale and offset as one value
+template <typename T> struct ScalePair {
+    typedef uint32_t type;
+    __device__ static type make(T s, T o) {
+        return (uint32_t)__builtin_bit_cast(uint16_t, s) | (uint32_t)__builtin_bit_cast(uint16_t, o) << 16;
+    }
+    __device__ static void split(type p, float& s, float& o) {
+        s = (float)__builtin_bit_cast(T, (uint16_t)p);
+        o = (float)__builtin_bit_cast(T, (uint16_t)(p >> 16));
+    }
+};
+template <> struct ScalePair<float> {
+    typedef float2 type;
+    __device__ static type make(float s, float o) { return make_float2(s, o); }
+    __device__ static void split(type p, float& s, float& o) { s = p.x; o = p.y; }
+};
+
+// A workgroup takes 16 * RT rows of the weights and 16 * MT rows of x; its waves take the 128-column blocks of the weights
+// in turn and add their sums up through LDS.  x is the A operand of v_mfma_f32_16x16x32, the codes are the B operand, so a
+// lane ends with its own weight row's sums for four rows of x, and a group's scale is one value per lane.
 //
 // Lane (r, q) loads 16 bytes of row r, the codes of columns 32 q .. 32 q + 31 (64 contiguous bytes a row and load); a 4 x 4
 // transposition of words between the four lanes of a row (four cross-row swaps) turns them into the operands of four
 // steps of 32 columns, columns 8 q .. 8 q + 7 each, so that a step never mixes two groups and the weights need no layout
 // of their own in memory.
 //
+// Scales and offsets go through LDS, a chunk of blocks at a time, read from memory row by row: loaded by the lane that needs
+// them they are 16 cache lines a load for 2 bytes of each, which the L1 has lost again when the next group's are read (measured at
+// n 16384, k 8192, group 64, m 1: codes alone 12.7 us, with scales loaded by lane 26.7 us).
+//
 // The operand holds 16 + code.  With c = sum x (16 + code) and X = sum x over a group (the same product with ones),
 // sum x w = scale c + (offset - 16 scale) X.
-template <typename T, int MT, int GROUP>
-__global__ __launch_bounds__(1024) void linear4_kernel(Lin4Args a) {
+//
+// The loads of the wave's next block are issued before the products of this one.  Loads return in order: x, which comes from the L2, is
+// asked for before the codes of the next block, which come from memory, or with its own block (MT == 1).
+template <typename T, int MT, int RT, int GROUP>
+__global__ __launch_bounds__(MT == 1 ? 1024 : 512) void linear4_kernel(Lin4Args a) {
     typedef XFrag<T> XF;
     typedef typename XF::E E;
     typedef Code16<E> C16;
@@ -103,94 +130,189 @@ __global__ __launch_bounds__(1024) void linear4_kernel(Lin4Args a) {
     constexpr int NG = 128 / GROUP;                          // groups of a block
     constexpr int SPG = GROUP / 32;                          // steps of a group
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = (int)(blockDim.x >> 6);
+    const int tid = threadIdx.x, lane = tid & 63, waves = (int)(blockDim.x >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 15, q = lane >> 4;
-    const int row = min((int)blockIdx.x * 16 + r, a.n - 1);  // (rows beyond the last repeat it and are not stored)
     const int64_t m0 = (int64_t)blockIdx.y * (16 * MT);
-    const int groups = a.k / GROUP, blocks = (a.k + 127) / 128;
-    const uint8_t* codes = a.codes + (int64_t)row * (a.k / 2);
-    const T* scales = reinterpret_cast<const T*>(a.scales) + (int64_t)row * groups;
-    const T* offsets = a.offsets ? reinterpret_cast<const T*>(a.offsets) + (int64_t)row * groups : nullptr;
+    const int groups = a.k / GROUP, full = a.k / 128;        // blocks that k fills
+    const bool has_off = a.offsets != nullptr;
+    const float s_mul = has_off ? -16.f : -24.f, o_mul = has_off ? 1.f : 0.f;
+    // byte offsets of the lane's rows from the first row of the workgroup (k < 2^26: they fit 32 bits)
+    const int64_t row0 = (int64_t)blockIdx.x * (16 * RT);
+    const uint8_t* codes = a.codes + row0 * (a.k / 2);
+    const T* scales = reinterpret_cast<const T*>(a.scales) + row0 * groups;
+    const T* offsets = has_off ? reinterpret_cast<const T*>(a.offsets) + row0 * groups : scales;
+    const int rows_here = (int)min((int64_t)(16 * RT), a.n - row0);
+    uint32_t code_at[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        code_at[t] = (uint32_t)min(16 * t + r, rows_here - 1) * (uint32_t)(a.k / 2) + 16 * q;    // (rows beyond the last repeat it and are not stored)
+    }
     const T* x[MT];
 #pragma unroll
     for (int t = 0; t < MT; ++t) x[t] = reinterpret_cast<const T*>(a.x) + min(m0 + 16 * t + r, a.m - 1) * a.x_stride + 8 * q;
 
-    struct Block { uint4 w; T s[NG], o[NG]; };
+    struct Block { uint4 w[RT]; };
+    struct XBlock { XF f[4][MT]; };
     auto load = [&](int blk, Block& b) {
-        const int col = min(128 * blk + 32 * q, a.k - 32);   // (a piece beyond the row belongs to a step that is skipped)
-        b.w = *reinterpret_cast<const uint4*>(codes + (col >> 1));
 #pragma unroll
-        for (int i = 0; i < NG; ++i) {
-            const int g = min(blk * NG + i, groups - 1);
-            b.s[i] = scales[g];
-            if (offsets) b.o[i] = offsets[g];
+        for (int t = 0; t < RT; ++t) {
+            b.w[t] = *reinterpret_cast<const uint4*>(codes + (code_at[t] + (uint32_t)blk * 64));
         }
     };
-    f32x4 y[MT];
+    auto load_x = [&](int blk, XBlock& b) {
 #pragma unroll
-    for (int t = 0; t < MT; ++t) y[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < MT; ++t) {
+            const T* p = x[t] + 128 * blk;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) b.f[i][t].load(p + 32 * i);
+        }
+    };
+    f32x4 y[RT][MT];
+#pragma unroll
+    for (int u = 0; u < RT; ++u)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) y[u][t] = f32x4{0.f, 0.f, 0.f, 0.f};
     const x8 ones = __builtin_bit_cast(x8, make_uint4(C16::ONES, C16::ONES, C16::ONES, C16::ONES));
+    // one constant in a vector, one in a scalar register: the and-or of a pair of codes is then one instruction
+    uint32_t mask = C16::MASK, base = C16::BASE;
+    asm("" : "+v"(mask));
+    asm("" : "+s"(base));
 
-    Block cur;
-    if (wave < blocks) load(wave, cur);
-    for (int blk = wave; blk < blocks; blk += waves) {
-        Block next;
-        if (blk + waves < blocks) load(blk + waves, next);
-        uint32_t w[4] = {cur.w.x, cur.w.y, cur.w.z, cur.w.w};
-        {
-            auto p = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
-            w[0] = p[0]; w[2] = p[1];
-            p = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
-            w[1] = p[0]; w[3] = p[1];
-            p = __builtin_amdgcn_permlane16_swap(w[0], w[1], false, false);
-            w[0] = p[0]; w[1] = p[1];
-            p = __builtin_amdgcn_permlane16_swap(w[2], w[3], false, false);
-            w[2] = p[0]; w[3] = p[1];
+    // [16 * RT rows][groups of the chunk], scale and offset side by side; an odd row stride spreads the 16 rows over the banks
+    typedef typename ScalePair<T>::type Pair;
+    Pair* pairs = reinterpret_cast<Pair*>(smem);
+    const int pair_stride = (a.chunk * NG) | 1;
+    // g0: the block's first group in the chunk
+    auto process = [&](const Block& cur, const XBlock& xcur, int g0, int steps) {
+        uint32_t w[RT][4];
+#pragma unroll
+        for (int u = 0; u < RT; ++u) {
+            auto p = __builtin_amdgcn_permlane32_swap(cur.w[u].x, cur.w[u].z, false, false);
+            w[u][0] = p[0]; w[u][2] = p[1];
+            p = __builtin_amdgcn_permlane32_swap(cur.w[u].y, cur.w[u].w, false, false);
+            w[u][1] = p[0]; w[u][3] = p[1];
+            p = __builtin_amdgcn_permlane16_swap(w[u][0], w[u][1], false, false);
+            w[u][0] = p[0]; w[u][1] = p[1];
+            p = __builtin_amdgcn_permlane16_swap(w[u][2], w[u][3], false, false);
+            w[u][2] = p[0]; w[u][3] = p[1];
         }
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-            if (blk * 128 + g * GROUP >= a.k) break;         // (k is a whole number of groups)
-            const float s = (float)cur.s[g];
-            const float off = (offsets ? (float)cur.o[g] : -8.f * s) - 16.f * s;
-            f32x4 c[MT], X[MT];
+            if (g * SPG >= steps) break;                     // (k is a whole number of groups)
+            f32x4 c[RT][MT], X[MT];
 #pragma unroll
-            for (int t = 0; t < MT; ++t) c[t] = X[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int t = 0; t < MT; ++t) {
+                X[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int u = 0; u < RT; ++u) c[u][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
 #pragma unroll
             for (int i = 0; i < SPG; ++i) {
                 const int step = g * SPG + i;
-                const x8 code = __builtin_bit_cast(x8, C16::unpack(w[step]));
+                x8 code[RT];
+#pragma unroll
+                for (int u = 0; u < RT; ++u) code[u] = __builtin_bit_cast(x8, C16::unpack(w[u][step], mask, base));
 #pragma unroll
                 for (int t = 0; t < MT; ++t) {
-                    XF xf;
-                    xf.load(x[t] + 128 * blk + 32 * step);
                     uint4 part[XF::PARTS];
-                    xf.parts(part);
+                    xcur.f[step][t].parts(part);
 #pragma unroll
                     for (int p = 0; p < XF::PARTS; ++p) {
                         const x8 xa = __builtin_bit_cast(x8, part[p]);
-                        c[t] = C16::mfma(xa, code, c[t]);
                         X[t] = C16::mfma(xa, ones, X[t]);
+#pragma unroll
+                        for (int u = 0; u < RT; ++u) c[u][t] = C16::mfma(xa, code[u], c[u][t]);
                     }
                 }
             }
 #pragma unroll
-            for (int t = 0; t < MT; ++t)
+            for (int u = 0; u < RT; ++u) {
+                float s, off;
+                ScalePair<T>::split(pairs[(16 * u + r) * pair_stride + g0 + g], s, off);
+                off = fmaf(s_mul, s, off * o_mul);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) y[t][i] = fmaf(s, c[t][i], fmaf(off, X[t][i], y[t][i]));
+                for (int t = 0; t < MT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) y[u][t][i] = fmaf(s, c[u][t][i], fmaf(off, X[t][i], y[u][t][i]));
+            }
         }
-        cur = next;
+    };
+
+    for (int c0 = 0; c0 * 128 < a.k; c0 += a.chunk) {
+        const int c_full = min(full, c0 + a.chunk);           // whole blocks [c0, c_full)
+        // a wave's blocks are neighbours: the two that share the 128-byte lines of a row follow each other
+        const int per = (c_full - c0 + waves - 1) / waves;
+        const int first = c0 + wave * per, last = min(c_full, first + per) - 1;
+        Block b0, b1;
+        XBlock x0, x1;
+        if (first <= last) {
+            if (MT == 1) load_x(first, x0);
+            load(first, b0);
+        }
+        {
+            const int g_first = c0 * NG, g_n = min(groups - g_first, a.chunk * NG);
+            const int total = rows_here * g_n;
+            for (int i = tid; i < total; i += 4 * (int)blockDim.x) {
+                T sv[4], ov[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int e = min(i + j * (int)blockDim.x, total - 1), row = e / g_n;
+                    const uint32_t at = (uint32_t)row * (uint32_t)groups + (uint32_t)(g_first + e - row * g_n);
+                    sv[j] = scales[at];
+                    ov[j] = offsets[at];
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int e = min(i + j * (int)blockDim.x, total - 1), row = e / g_n;
+                    pairs[row * pair_stride + e - row * g_n] = ScalePair<T>::make(sv[j], ov[j]);
+                }
+            }
+        }
+        __syncthreads();
+        for (int blk = first; blk <= last; blk += 2) {
+            const int second = min(blk + 1, last), third = min(blk + 2, last);
+            if (MT == 1) load_x(second, x1);
+            else load_x(blk, x0);
+            __builtin_amdgcn_sched_barrier(0);
+            load(second, b1);
+            __builtin_amdgcn_sched_barrier(0);
+            process(b0, x0, (blk - c0) * NG, 4);
+            if (blk == last) break;
+            if (MT == 1) load_x(third, x0);
+            else load_x(second, x1);
+            __builtin_amdgcn_sched_barrier(0);
+            load(third, b0);
+            __builtin_amdgcn_sched_barrier(0);
+            process(b1, x1, (second - c0) * NG, 4);
+        }
+        // the last block of a row that ends inside it, by the last wave: pieces beyond the row are loaded from its last 32
+        // columns and belong to steps that are not taken
+        if (a.k % 128 != 0 && full < c0 + a.chunk && wave == waves - 1) {
+            const int col = min(128 * full + 32 * q, a.k - 32);
+#pragma unroll
+            for (int t = 0; t < RT; ++t) b0.w[t] = *reinterpret_cast<const uint4*>(codes + (code_at[t] - 16 * q + (uint32_t)(col >> 1)));
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int t = 0; t < MT; ++t) x0.f[i][t].load(x[t] + min(128 * full + 32 * i, a.k - 32));
+            process(b0, x0, (full - c0) * NG, (a.k % 128) / 32);
+        }
+        __syncthreads();                                     // the scales are read: the next chunk's, or the sums, go there
     }
 
     // the waves' sums, in the order of the waves
-    f32x4* part = reinterpret_cast<f32x4*>(smem);            // [waves][MT][64]
+    f32x4* part = reinterpret_cast<f32x4*>(smem);            // [waves][RT][MT][64]
 #pragma unroll
-    for (int t = 0; t < MT; ++t) part[(wave * MT + t) * 64 + lane] = y[t];
+    for (int u = 0; u < RT; ++u)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) part[((wave * RT + u) * MT + t) * 64 + lane] = y[u][t];
     __syncthreads();
-    for (int i = tid; i < MT * 64; i += (int)blockDim.x) {
+    for (int i = tid; i < RT * MT * 64; i += (int)blockDim.x) {
         f32x4 sum = part[i];
-        for (int v = 1; v < waves; ++v) sum += part[v * MT * 64 + i];
-        const int n = (int)blockIdx.x * 16 + (i & 15);
-        const int64_t m = m0 + 16 * (i >> 6) + 4 * ((i & 63) >> 4);
+        for (int v = 1; v < waves; ++v) sum += part[v * RT * MT * 64 + i];
+        const int n = ((int)blockIdx.x * RT + i / (MT * 64)) * 16 + (i & 15);
+        const int64_t m = m0 + 16 * ((i / 64) % MT) + 4 * ((i & 63) >> 4);
         if (n >= a.n) continue;
         const float bias = a.bias ? (float)reinterpret_cast<const T*>(a.bias)[n] : 0.f;
 #pragma unroll
@@ -199,27 +321,36 @@ __global__ __launch_bounds__(1024) void linear4_kernel(Lin4Args a) {
     }
 }
 
-template <typename T, int MT>
-int linear4_by_group(const Lin4Args& a, hipStream_t stream) {
-    const int tiles = (a.n + 15) / 16, blocks = (a.k + 127) / 128;
+template <typename T, int MT, int RT>
+int linear4_by_group(Lin4Args a, hipStream_t stream) {
+    const int tiles = (a.n + 16 * RT - 1) / (16 * RT), blocks = (a.k + 127) / 128;
     const int64_t my = ceil_div64(a.m, 16 * MT);
     RAG_REQUIRE(my <= 65535, RAG_ELIMIT, "rag_enc_linear4: too many rows of x");
     int waves = 4;
-    while (waves < 16 && waves < blocks && (int64_t)tiles * my * waves < 4096) waves *= 2;
+    while (waves < (MT == 1 ? 16 : 8) && waves < blocks && (int64_t)tiles * my * waves < 4096) waves *= 2;
     const dim3 grid((unsigned)tiles, (unsigned)my);
-    const size_t lds = (size_t)waves * MT * 1024;
-    if (a.group == 32) linear4_kernel<T, MT, 32><<<grid, 64 * waves, lds, stream>>>(a);
-    else if (a.group == 64) linear4_kernel<T, MT, 64><<<grid, 64 * waves, lds, stream>>>(a);
-    else linear4_kernel<T, MT, 128><<<grid, 64 * waves, lds, stream>>>(a);
+    // at most 32 KB of scales at a time
+    const int ng = 128 / a.group, row_bytes = 16 * RT * (int)sizeof(typename ScalePair<T>::type);
+    a.chunk = std::min(blocks, 32768 / (row_bytes * ng));
+    const size_t lds = std::max((size_t)row_bytes * ((a.chunk * ng) | 1), (size_t)waves * MT * RT * 1024);
+    if (a.group == 32) linear4_kernel<T, MT, RT, 32><<<grid, 64 * waves, lds, stream>>>(a);
+    else if (a.group == 64) linear4_kernel<T, MT, RT, 64><<<grid, 64 * waves, lds, stream>>>(a);
+    else linear4_kernel<T, MT, RT, 128><<<grid, 64 * waves, lds, stream>>>(a);
     RAG_HIP_TRY(hipGetLastError());
     return RAG_OK;
 }
 
+template <typename T, int MT>
+int linear4_by_rows(const Lin4Args& a, hipStream_t stream) {
+    if (a.n >= 8192) return linear4_by_group<T, MT, 2>(a, stream);
+    return linear4_by_group<T, MT, 1>(a, stream);
+}
+
 template <typename T>
 int linear4_launch(const Lin4Args& a, hipStream_t stream) {
-    if (a.m <= 16) return linear4_by_group<T, 1>(a, stream);
-    if (a.m <= 32) return linear4_by_group<T, 2>(a, stream);
-    return linear4_by_group<T, 4>(a, stream);
+    if (a.m <= 16) return linear4_by_rows<T, 1>(a, stream);
+    if (a.m <= 32) return linear4_by_rows<T, 2>(a, stream);
+    return linear4_by_rows<T, 4>(a, stream);
 }
 
 }  // namespace
@@ -232,7 +363,7 @@ extern "C" int rag_enc_linear4_dev(const void* d_x, int64_t x_stride, const uint
     RAG_REQUIRE(m >= 0 && n >= 1 && k >= 1, RAG_EINVAL, "%s: bad sizes", me);
     RAG_REQUIRE(group == 32 || group == 64 || group == 128, RAG_ELIMIT, "%s: the group must be 32, 64 or 128 (got %d)", me, group);
     RAG_REQUIRE(k % group == 0, RAG_ELIMIT, "%s: k = %d is not a multiple of the group %d", me, k, group);
-    RAG_REQUIRE(m < (1ll << 31) && n < (1 << 30) && k < (1 << 30), RAG_ELIMIT, "%s: sizes beyond the limit", me);
+    RAG_REQUIRE(m < (1ll << 31) && n < (1 << 30) && k < (1 << 26), RAG_ELIMIT, "%s: sizes beyond the limit", me);
     if (m == 0) return RAG_OK;
     RAG_REQUIRE(d_x && d_codes && d_scales && d_y, RAG_EINVAL, "%s: null pointer", me);
     const int size = dtype == RAG_DTYPE_F32 ? 4 : 2;
@@ -242,7 +373,7 @@ extern "C" int rag_enc_linear4_dev(const void* d_x, int64_t x_stride, const uint
                 reinterpret_cast<uintptr_t>(d_bias) % size == 0 && reinterpret_cast<uintptr_t>(d_y) % size == 0, RAG_EINVAL,
                 "%s: misaligned pointer", me);
     RAG_REQUIRE((m == 1 || x_stride >= k) && (m == 1 || y_stride >= n), RAG_EINVAL, "%s: a row's stride is smaller than the row", me);
-    Lin4Args a{d_x, d_codes, d_scales, d_offsets, d_bias, d_y, x_stride, y_stride, m, n, k, group};
+    Lin4Args a{d_x, d_codes, d_scales, d_offsets, d_bias, d_y, x_stride, y_stride, m, n, k, group, 0};
     hipStream_t stream = (hipStream_t)stream_;
     if (dtype == RAG_DTYPE_F32) return linear4_launch<float>(a, stream);
     if (dtype == RAG_DTYPE_BF16) return linear4_launch<bf16>(a, stream);
