@@ -86,6 +86,9 @@ template <> struct XFrag<float> {
     }
 };
 
+// (1024 threads leave 128 registers a lane: enough for one row tile of 16-bit x)
+template <typename T, int MT> constexpr int max_waves() { return MT == 1 && sizeof(T) == 2 ? 16 : 8; }
+
 // A group's scale and offset as one value
 template <typename T> struct ScalePair {
     typedef uint32_t type;
@@ -122,7 +125,7 @@ template <> struct ScalePair<float> {
 // The loads of the wave's next block are issued before the products of this one.  Loads return in order: x, which comes from the L2, is
 // asked for before the codes of the next block, which come from memory, or with its own block (MT == 1).
 template <typename T, int MT, int RT, int GROUP>
-__global__ __launch_bounds__(MT == 1 ? 1024 : 512) void linear4_kernel(Lin4Args a) {
+__global__ __launch_bounds__((64 * max_waves<T, MT>())) void linear4_kernel(Lin4Args a) {
     typedef XFrag<T> XF;
     typedef typename XF::E E;
     typedef Code16<E> C16;
@@ -327,7 +330,7 @@ int linear4_by_group(Lin4Args a, hipStream_t stream) {
     const int64_t my = ceil_div64(a.m, 16 * MT);
     RAG_REQUIRE(my <= 65535, RAG_ELIMIT, "rag_enc_linear4: too many rows of x");
     int waves = 4;
-    while (waves < (MT == 1 ? 16 : 8) && waves < blocks && (int64_t)tiles * my * waves < 4096) waves *= 2;
+    while (waves < max_waves<T, MT>() && waves < blocks && (int64_t)tiles * my * waves < 4096) waves *= 2;
     const dim3 grid((unsigned)tiles, (unsigned)my);
     // at most 32 KB of scales at a time
     const int ng = 128 / a.group, row_bytes = 16 * RT * (int)sizeof(typename ScalePair<T>::type);

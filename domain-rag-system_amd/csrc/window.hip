@@ -9,6 +9,7 @@
 #include "common.h"
 
 #include <math.h>
+#include <stdlib.h>
 
 namespace {
 
@@ -85,7 +86,6 @@ __device__ void attend_row(const WinArgs& a, const Seq& sq, int j, int head, int
             s = dot * a.scale;
         }
         float mx = s;
-        bool bad = s != s;                                   // fmaxf would drop a NaN
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
         const float m_new = fmaxf(m, mx);
@@ -94,7 +94,6 @@ __device__ void attend_row(const WinArgs& a, const Seq& sq, int j, int head, int
         float sum = lane < n ? p : 0.f;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
-        (void)bad;
         const float alpha = exp2f(m - top);
         l = l * alpha + sum;
         o0 *= alpha;
@@ -121,22 +120,299 @@ __device__ void attend_row(const WinArgs& a, const Seq& sq, int j, int head, int
     }
 }
 
-template <typename T, int D>
-__global__ __launch_bounds__(256) void window_row_kernel(WinArgs a, uint32_t* fault) {
-    const int rows4 = (a.max_q + 3) / 4;
-    const int seq = (int)(blockIdx.x / rows4);
-    const int j = (int)(blockIdx.x % rows4) * 4 + (int)(threadIdx.x >> 6);
-    const int head = (int)blockIdx.y;
-    Seq s;
-    if (!load_seq(a, seq, s, fault) || j >= s.nq) return;
-    attend_row<T, D>(a, s, j, head, threadIdx.x & 63);
+// ---- a tile of 128 queries of one head per workgroup -------------------------------------------------
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ float both_halves_max(float v) {
+    const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+}
+__device__ __forceinline__ float both_halves_sum(float v) {
+    const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+}
+__device__ __forceinline__ void trade_halves(uint32_t& a, uint32_t& b) {
+    const auto p = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+    a = p[0];
+    b = p[1];
+}
+
+// One wave-instruction of a direct-to-LDS load: lane l's 16 bytes at gbase + voff land at LDS byte lds_dst + 16 l.  M0
+// carries the destination and belongs to the compiler, so it is saved and restored inside the statement.  The compiler
+// does not count this load: wait with s_waitcnt vmcnt before reading.
+__device__ __forceinline__ void lds_dma16(uint32_t lds_dst, const void* gbase, uint32_t voff) {
+    unsigned keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep) : "v"(voff), "s"(lds_dst), "s"(gbase) : "memory");
+}
+
+// The image of a tile of keys or values in LDS: rows of D elements, the 16-byte piece p of row `key` at place
+// p ^ swizzle(key), so that neither the rows that a matrix operand reads at one piece nor the blocks that the
+// transposing read takes fall on the same banks.
+template <typename E, int D> struct Image {
+    static constexpr int ROWB = D * (int)sizeof(E);          // bytes of a row
+    static constexpr int PIECES = ROWB / 16;
+    static constexpr int KT = sizeof(E) == 4 ? 32 : 64;      // keys of a tile
+    static constexpr int BYTES = KT * ROWB;
+    // 16 neighbouring rows at one piece index cover all banks once
+    __device__ static int k_swizzle(int row) {
+        return PIECES >= 16 ? row & 15 : PIECES == 8 ? (row >> 1) & 7 : (row >> 2) & 3;
+    }
+    // 16 bits: 4 neighbouring rows x 4 neighbouring pieces; 32 bits: rows 4 apart, 8 pieces
+    __device__ static int v_swizzle(int row) {
+        if (sizeof(E) == 4) return PIECES >= 16 ? ((row >> 2) & 1) << 3 : 0;
+        return PIECES == 16 ? (row & 3) << 2 | ((row >> 2) & 3) : PIECES == 8 ? ((row >> 1) & 1) << 2 | ((row >> 2) & 3) : 0;
+    }
+};
+
+template <typename E> struct Mma;
+template <> struct Mma<bf16> {
+    typedef typename Vec<bf16, 8>::type x8;
+    __device__ static f32x16 mfma(x8 a, x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct Mma<f16> {
+    typedef typename Vec<f16, 8>::type x8;
+    __device__ static f32x16 mfma(x8 a, x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+
+constexpr float NEG_BIG = -1e30f;    // the running maximum's start: finite, so that no difference of infinities arises
+constexpr float LAG = 8.f;           // the maximum may lag behind by this power of two before the sums are rescaled
+
+// Four waves, each 32 queries (the columns of the matrix products) of a 128-query tile of one head; tiles of keys and values
+// come into LDS by direct loads, two buffers, the next tile's loads in flight while this one is worked on, one barrier a tile.
+//   S^T = K Q^T        rows = keys, a lane holds 16 keys (registers, lane half) of its query (lane % 32)
+//   O^T += V^T P^T     the lane's probabilities are the B operand as they stand; V^T comes out of the row-major image
+//                      through the transposing LDS read (16 bits) or by single values (fp32)
+// 16-bit types: probabilities are rounded to the type (half a step of each, which the sum in fp32 does not see), fp32
+// sums.  fp32: v_mfma_f32_32x32x2_f32, exact fp32 products.
+// The running maximum is only raised when a score exceeds it by 2^LAG (the probabilities then stay below 2^LAG, exact in
+// every type), so that the rescaling of the sums is rare.
+// Masked scores are -infinity; a tile that every query of the wave sees whole needs no mask.  Where keys or
+// values hold infinities or NaN, 0 * infinity spoils rows that do not see them: every row that ends as NaN is computed
+// again by attend_row, which reads only what the row sees.
+template <typename E, int D>
+__global__ __launch_bounds__(256, sizeof(E) == 4 ? 1 : 2) void window_tile_kernel(WinArgs a, int q_tiles, int64_t units, uint32_t* fault) {
+    typedef Image<E, D> I;
+    constexpr int KT = I::KT, KB = KT / 32, DT = D / 32, KC = I::PIECES / 2;
+    extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    // the units of one (sequence, key/value head) are neighbours, and an eighth of them all goes to each L2
+    const int64_t unit = (int64_t)(blockIdx.x & 7) * ((units + 7) >> 3) + (blockIdx.x >> 3);
+    if ((blockIdx.x >> 3) >= ((units + 7) >> 3) || unit >= units) return;
+    const int group = a.hq / a.hkv;
+    const int g = (int)(unit % group);
+    const int64_t u1 = unit / group;
+    const int qt = q_tiles - 1 - (int)(u1 % q_tiles);        // (a causal sequence's last tiles are its longest)
+    const int64_t u2 = u1 / q_tiles;
+    const int kvh = (int)(u2 % a.hkv), seq = (int)(u2 / a.hkv);
+    const int head = kvh * group + g;
+    Seq sq;
+    if (!load_seq(a, seq, sq, fault) || qt * 128 >= sq.nq) return;
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 31, h = lane >> 5;
+    const int q0 = qt * 128 + wave * 32;                     // first query of the wave
+    const int qr = q0 + r;
+    const bool wave_on = q0 < sq.nq, row_on = qr < sq.nq;
+    const int shift = sq.nk - sq.nq;                         // position of query 0
+    const Seen mine = seen_by(a, shift + min(qr, sq.nq - 1), sq.nk);
+    const Seen w_first = seen_by(a, shift + q0, sq.nk), w_last = seen_by(a, shift + min(q0 + 31, sq.nq - 1), sq.nk);
+    const Seen t_first = seen_by(a, shift + qt * 128, sq.nk), t_last = seen_by(a, shift + min(qt * 128 + 127, sq.nq - 1), sq.nk);
+    // the tiles of keys that some query of the workgroup sees
+    const int sink_tiles = (min(a.sinks, t_first.lo) + KT - 1) / KT;
+    const int win_tile = max(sink_tiles, t_first.lo / KT);
+    const int n_tiles = sink_tiles + max(0, (t_last.hi + KT - 1) / KT - win_tile);
+
+    const unsigned char* kbase = reinterpret_cast<const unsigned char*>(a.k) + (sq.k0 * a.k_row + (int64_t)kvh * a.k_head) * (int64_t)sizeof(E);
+    const unsigned char* vbase = reinterpret_cast<const unsigned char*>(a.v) + (sq.k0 * a.v_row + (int64_t)kvh * a.v_head) * (int64_t)sizeof(E);
+    const uint32_t k_rowb = (uint32_t)(a.k_row * (int64_t)sizeof(E)), v_rowb = (uint32_t)(a.v_row * (int64_t)sizeof(E));
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
+    auto first_key = [&](int t) { return (t < sink_tiles ? t : win_tile + t - sink_tiles) * KT; };
+    auto stage = [&](int t) {
+        const int key0 = first_key(t);
+        const int last = sq.nk - 1 - key0;                   // rows beyond the last key repeat it (masked)
+        const unsigned char *kp = kbase + (int64_t)key0 * k_rowb, *vp = vbase + (int64_t)key0 * v_rowb;
+        const uint32_t dst = lds0 + (t & 1) * 2 * I::BYTES;
+#pragma unroll
+        for (int j = 0; j < I::BYTES / 4096; ++j) {
+            const int n = wave + 4 * j, o = n * 1024 + lane * 16;
+            const int row = o / I::ROWB, place = (o % I::ROWB) / 16;
+            const uint32_t src = (uint32_t)min(row, last);
+            lds_dma16(dst + n * 1024, kp, src * k_rowb + (place ^ I::k_swizzle(row)) * 16);
+            lds_dma16(dst + I::BYTES + n * 1024, vp, src * v_rowb + (place ^ I::v_swizzle(row)) * 16);
+        }
+    };
+    if (n_tiles > 0) stage(0);
+
+    // Q^T: piece 2c + h of the lane's query
+    const bool flip = a.scale < 0.f;                         // a negative scale goes into q: the maximum is taken of products as they are
+    const float scale = fabsf(a.scale);
+    u32x4 qf[KC];
+    {
+        const unsigned char* qp = reinterpret_cast<const unsigned char*>(a.q) + ((sq.q0 + min(qr, sq.nq - 1)) * a.q_stride + (int64_t)head * D) * (int64_t)sizeof(E);
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+            qf[c] = *reinterpret_cast<const u32x4*>(qp + (2 * c + h) * 16);
+            if (flip) qf[c] ^= sizeof(E) == 4 ? 0x80000000u : 0x80008000u;
+        }
+    }
+    float m_run = NEG_BIG, l_run = 0.f;                      // l_run: the lane's own keys
+    f32x16 o[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
+
+    for (int t = 0; t < n_tiles; ++t) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // this tile's loads
+        __syncthreads();
+        if (t + 1 < n_tiles) stage(t + 1);
+        const int key0 = first_key(t);
+        const bool some = wave_on && key0 < w_last.hi && (key0 + KT > w_first.lo || key0 < a.sinks);
+        if (!some) continue;
+        const unsigned char* ks = smem + (t & 1) * 2 * I::BYTES;
+        const unsigned char* vs = ks + I::BYTES;
+        f32x16 s[KB];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[kb][i] = 0.f;
+#pragma unroll
+            for (int c = 0; c < KC; ++c) {
+                const u32x4 kf = *reinterpret_cast<const u32x4*>(ks + (kb * 32 + r) * I::ROWB + ((2 * c + h) ^ I::k_swizzle(r)) * 16);
+                if constexpr (sizeof(E) == 4) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        s[kb] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kf[j]), __uint_as_float(qf[c][j]), s[kb], 0, 0, 0);
+                } else {
+                    s[kb] = Mma<E>::mfma(__builtin_bit_cast(typename Mma<E>::x8, kf), __builtin_bit_cast(typename Mma<E>::x8, qf[c]), s[kb]);
+                }
+            }
+        }
+        const bool whole = key0 + KT <= w_first.hi && (key0 >= w_last.lo || key0 + KT <= a.sinks);
+        if (!whole) {
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int key = key0 + 32 * kb + 8 * (i >> 2) + 4 * h + (i & 3);
+                    const bool seen = key < mine.hi && (key >= mine.lo || key < mine.s);
+                    s[kb][i] = seen ? s[kb][i] : -INFINITY;
+                }
+        }
+        float mx = NEG_BIG;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
+        mx = both_halves_max(mx);
+        if (__any((mx - m_run) * scale > LAG)) {
+            const float m_new = fmaxf(m_run, mx);
+            const float alpha = __builtin_amdgcn_exp2f((m_run - m_new) * scale);
+            m_run = m_new;
+            l_run *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[dt][i] *= alpha;
+        }
+        const float ms = m_run * scale;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[kb][i] = __builtin_amdgcn_exp2f(fmaf(s[kb][i], scale, -ms));
+                l_run += s[kb][i];
+            }
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            if constexpr (sizeof(E) == 4) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int key = 32 * kb + 8 * (i >> 2) + 4 * h + (i & 3);
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) {
+                        const float v = *reinterpret_cast<const float*>(vs + key * I::ROWB + (((dt * 8 + (r >> 2)) ^ I::v_swizzle(key)) * 16) + (r & 3) * 4);
+                        o[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, s[kb][i], o[dt], 0, 0, 0);
+                    }
+                }
+            } else {
+                typedef short tr4 __attribute__((__vector_size__(4 * sizeof(short))));
+                const int rho = (lane & 15) >> 2, col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+#pragma unroll
+                for (int tt = 0; tt < 2; ++tt) {
+                    typename Mma<E>::x8 pb;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) pb[j] = (E)s[kb][8 * tt + j];
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) {
+                        union { tr4 t[2]; typename Mma<E>::x8 v; } av;
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            const int row = 32 * kb + 16 * tt + 8 * u + 4 * h + rho;
+                            const unsigned char* p = vs + row * I::ROWB + (((dt * 4 + (col >> 3)) ^ I::v_swizzle(row)) * 16) + (col & 4) * 2;
+                            av.t[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) tr4*)p);
+                        }
+                        o[dt] = Mma<E>::mfma(av.v, pb, o[dt]);
+                    }
+                }
+            }
+        }
+    }
+    if (!wave_on) return;
+
+    const bool any_seen = mine.s + (mine.hi - mine.lo) > 0;
+    const float inv = 1.f / both_halves_sum(l_run);
+    bool bad = false;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            o[dt][i] = any_seen ? o[dt][i] * inv : 0.f;
+            bad |= o[dt][i] != o[dt][i];
+        }
+    const uint64_t bad64 = __ballot(bad && row_on);
+    const uint32_t bad_rows = (uint32_t)bad64 | (uint32_t)(bad64 >> 32);
+    const bool store = row_on && !(bad_rows >> r & 1);
+    E* dst = reinterpret_cast<E*>(a.out) + (sq.q0 + qr) * a.out_stride + (int64_t)head * D;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+        if constexpr (sizeof(E) == 4) {
+            if (store)
+#pragma unroll
+                for (int gq = 0; gq < 4; ++gq)
+                    *reinterpret_cast<float4*>(dst + dt * 32 + 8 * gq + 4 * h) = make_float4(o[dt][4 * gq], o[dt][4 * gq + 1], o[dt][4 * gq + 2], o[dt][4 * gq + 3]);
+        } else {
+            // the two lanes of a query trade halves of their groups, so that a lane stores 16 neighbouring bytes
+            uint2 grp[4];
+#pragma unroll
+            for (int gq = 0; gq < 4; ++gq) {
+                typename Vec<E, 4>::type v;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = (E)o[dt][4 * gq + j];
+                grp[gq] = __builtin_bit_cast(uint2, v);
+            }
+            trade_halves(grp[0].x, grp[1].x); trade_halves(grp[0].y, grp[1].y);
+            trade_halves(grp[2].x, grp[3].x); trade_halves(grp[2].y, grp[3].y);
+            if (store) {
+                *reinterpret_cast<uint4*>(dst + dt * 32 + 8 * h) = make_uint4(grp[0].x, grp[0].y, grp[1].x, grp[1].y);
+                *reinterpret_cast<uint4*>(dst + dt * 32 + 8 * h + 16) = make_uint4(grp[2].x, grp[2].y, grp[3].x, grp[3].y);
+            }
+        }
+    }
+    for (uint32_t rest = bad_rows; rest != 0; rest &= rest - 1) attend_row<E, D>(a, sq, q0 + __builtin_ctz(rest), head, lane);
 }
 
 template <typename T, int D>
 int window_launch(const WinArgs& a, hipStream_t stream) {
-    const int64_t grid = (int64_t)a.n_seq * ((a.max_q + 3) / 4);
-    RAG_REQUIRE(grid < (1ll << 31), RAG_ELIMIT, "rag_enc_attention_window: too many query rows");
-    window_row_kernel<T, D><<<dim3((unsigned)grid, (unsigned)a.hq), 256, 0, stream>>>(a, rag_fault_word());
+    const int q_tiles = (a.max_q + 127) / 128;
+    const int64_t units = (int64_t)a.n_seq * q_tiles * a.hq;
+    const int64_t grid = (units + 7) / 8 * 8;
+    RAG_REQUIRE(grid < (1ll << 31), RAG_ELIMIT, "rag_enc_attention_window: too many query tiles");
+    constexpr size_t lds = 4 * (size_t)Image<T, D>::BYTES;
+    RAG_GRANT_LDS((window_tile_kernel<T, D>), lds);
+    window_tile_kernel<T, D><<<(unsigned)grid, 256, lds, stream>>>(a, q_tiles, units, rag_fault_word());
     RAG_HIP_TRY(hipGetLastError());
     return RAG_OK;
 }
@@ -184,6 +460,8 @@ extern "C" int rag_enc_attention_window_dev(const void* d_q, int64_t q_stride, c
                 v_head_stride * size % 16 == 0 && out_stride * size % 16 == 0, RAG_EINVAL, "%s: strides must be multiples of 16 bytes", me);
     RAG_REQUIRE(q_stride >= (int64_t)n_q_heads * head_dim && out_stride >= (int64_t)n_q_heads * head_dim, RAG_EINVAL,
                 "%s: a row's stride is smaller than the row", me);
+    RAG_REQUIRE(llabs(k_row_stride) * size <= (1 << 25) && llabs(v_row_stride) * size <= (1 << 25) && k_row_stride >= 0 && v_row_stride >= 0, RAG_ELIMIT,
+                "%s: rows of keys and values lie at most 32 MB apart", me);
     RAG_REQUIRE(workspace_bytes >= 0, RAG_EINVAL, "%s: bad workspace", me);
     WinArgs a;
     a.q = d_q; a.k = d_k; a.v = d_v; a.out = d_out; a.cu_q = d_cu_q; a.k_start = d_k_start; a.k_len = d_k_len;
