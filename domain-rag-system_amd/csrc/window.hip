@@ -8,6 +8,8 @@
 // that is, the keys [0, s) and [lo, hi) of Seen below.  out = sum softmax(scale q.k) v over them; none: 0.
 #include "common.h"
 
+#include <algorithm>
+
 #include <math.h>
 #include <stdlib.h>
 
@@ -404,8 +406,410 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 ? 1 : 2) void window_tile_kerne
     for (uint32_t rest = bad_rows; rest != 0; rest &= rest - 1) attend_row<E, D>(a, sq, q0 + __builtin_ctz(rest), head, lane);
 }
 
+// ---- few queries over many keys ------------------------------------------------------------------
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// The rows of one key/value head's queries (row = query * group + head of the group) are the columns of the matrix
+// products, 16 * QT of them per workgroup, so that a key is read once for all of them.  Four waves take tiles of keys in turn,
+// each into its own two LDS buffers (no barrier until the end), and put their results together; a long text is cut
+// into spans of `span` tiles, one workgroup each, whose results window_join_kernel puts together.
+// Bound by the bytes of the keys and values: 64 KB of loads are in flight per compute unit.
+template <typename E, int D> struct FewImage {
+    static constexpr int ROWB = D * (int)sizeof(E);
+    static constexpr int PIECES = ROWB / 16;
+    static constexpr int KT = sizeof(E) == 4 ? 16 : 32;      // keys of a wave's tile
+    static constexpr int BYTES = KT * ROWB;
+    __device__ static int k_swizzle(int row) { return Image<E, D>::k_swizzle(row); }
+    // 16 bits: 8 neighbouring rows x 2 neighbouring pieces; 32 bits: rows 4 apart, 4 pieces
+    __device__ static int v_swizzle(int row) {
+        if (sizeof(E) == 4) return PIECES >= 16 ? ((row >> 2) & 3) << 2 : ((row >> 2) & 1) << 2;
+        return PIECES == 16 ? (row & 7) << 1 : PIECES == 8 ? ((row >> 1) & 3) << 1 : ((row >> 2) & 1) << 1;
+    }
+};
+
+template <typename E> struct MmaFew;
+template <> struct MmaFew<bf16> {
+    __device__ static f32x4 mfma(Mma<bf16>::x8 a, Mma<bf16>::x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct MmaFew<f16> {
+    __device__ static f32x4 mfma(Mma<f16>::x8 a, Mma<f16>::x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+
+// The tiles of `kt` keys that queries j0 .. j1 of a sequence see: `sinks` from the text's start, then `window` from tile w0.
+struct Tiles {
+    int sinks, w0, n;
+    __device__ int first_key(int t, int kt) const { return (t < sinks ? t : w0 + t - sinks) * kt; }
+};
+__device__ __forceinline__ Tiles tiles_of(const WinArgs& a, const Seq& sq, int j0, int j1, int kt) {
+    const Seen first = seen_by(a, sq.nk - sq.nq + j0, sq.nk), last = seen_by(a, sq.nk - sq.nq + j1, sq.nk);
+    Tiles t;
+    t.sinks = (min(a.sinks, first.lo) + kt - 1) / kt;
+    t.w0 = max(t.sinks, first.lo / kt);
+    t.n = t.sinks + max(0, (last.hi + kt - 1) / kt - t.w0);
+    return t;
+}
+
+__device__ __forceinline__ float quarters_max(float v) {     // over the four lanes that share lane % 16
+    const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+    const auto q = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
+}
+__device__ __forceinline__ float quarters_sum(float v) {
+    const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+    const auto q = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(q[0]) + __uint_as_float(q[1]);
+}
+
+struct FewArgs {
+    int chunks;                      // of 16 * QT rows
+    int spans, span;                 // workgroups along the keys, tiles of each
+    float2* part_ml;                 // [query row * head][spans]: maximum, sum
+    float* part_o;                   // [query row * head][spans][D]
+};
+
+template <typename E, int D, int QT>
+__global__ __launch_bounds__(256) void window_few_kernel(WinArgs a, FewArgs f, uint32_t* fault) {
+    typedef FewImage<E, D> I;
+    constexpr int KT = I::KT, KB = KT / 16, DT = D / 16, KC = I::PIECES / 4, ROWS = 16 * QT;
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];       // [4 waves][2 buffers][K | V], later [4][ROWS][D] sums; [4][ROWS] (m, l)
+    const int group = a.hq / a.hkv;
+    const int64_t unit = blockIdx.x;
+    const int kvh = (int)(unit % a.hkv);
+    const int64_t u1 = unit / a.hkv;
+    const int chunk = (int)(u1 % f.chunks);
+    const int64_t u2 = u1 / f.chunks;
+    const int span = (int)(u2 % f.spans), seq = (int)(u2 / f.spans);
+    Seq sq;
+    if (!load_seq(a, seq, sq, fault)) return;
+    const int rows = min(ROWS, sq.nq * group - chunk * ROWS);
+    if (rows <= 0) return;
+    const int j0 = chunk * ROWS / group, j1 = (chunk * ROWS + rows - 1) / group;
+    const Tiles tiles = tiles_of(a, sq, j0, j1, KT);
+    const int t0 = span * f.span, t1 = min(tiles.n, t0 + f.span);
+    if (t0 >= t1 && span > 0) return;
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 15, g = lane >> 4;
+    const unsigned char* kbase = reinterpret_cast<const unsigned char*>(a.k) + (sq.k0 * a.k_row + (int64_t)kvh * a.k_head) * (int64_t)sizeof(E);
+    const unsigned char* vbase = reinterpret_cast<const unsigned char*>(a.v) + (sq.k0 * a.v_row + (int64_t)kvh * a.v_head) * (int64_t)sizeof(E);
+    const uint32_t k_rowb = (uint32_t)(a.k_row * (int64_t)sizeof(E)), v_rowb = (uint32_t)(a.v_row * (int64_t)sizeof(E));
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem + wave * 4 * I::BYTES;
+    const unsigned char* mine = smem + wave * 4 * I::BYTES;
+    constexpr int DMAS = I::BYTES / 1024;
+    auto stage = [&](int t, int buf) {
+        const int key0 = tiles.first_key(t, KT);
+        const int last = sq.nk - 1 - key0;
+        const unsigned char *kp = kbase + (int64_t)key0 * k_rowb, *vp = vbase + (int64_t)key0 * v_rowb;
+        const uint32_t dst = lds0 + buf * 2 * I::BYTES;
+#pragma unroll
+        for (int n = 0; n < DMAS; ++n) {
+            const int o = n * 1024 + lane * 16;
+            const int row = o / I::ROWB, place = (o % I::ROWB) / 16;
+            lds_dma16(dst + n * 1024, kp, (uint32_t)min(row, last) * k_rowb + (place ^ I::k_swizzle(row)) * 16);
+        }
+#pragma unroll
+        for (int n = 0; n < DMAS; ++n) {
+            const int o = n * 1024 + lane * 16;
+            const int row = o / I::ROWB, place = (o % I::ROWB) / 16;
+            lds_dma16(dst + I::BYTES + n * 1024, vp, (uint32_t)min(row, last) * v_rowb + (place ^ I::v_swizzle(row)) * 16);
+        }
+    };
+
+    const bool flip = a.scale < 0.f;
+    const float scale = fabsf(a.scale);
+    u32x4 qf[QT][KC];
+    Seen seen[QT];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+        const int row = chunk * ROWS + min(16 * qt + r, rows - 1), j = row / group, head = kvh * group + row % group;
+        seen[qt] = seen_by(a, sq.nk - sq.nq + j, sq.nk);
+        const unsigned char* qp = reinterpret_cast<const unsigned char*>(a.q) + ((sq.q0 + j) * a.q_stride + (int64_t)head * D) * (int64_t)sizeof(E);
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+            qf[qt][c] = *reinterpret_cast<const u32x4*>(qp + (4 * c + g) * 16);
+            if (flip) qf[qt][c] ^= sizeof(E) == 4 ? 0x80000000u : 0x80008000u;
+        }
+    }
+    float m[QT], l[QT];
+    f32x4 o[QT][DT];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+        m[qt] = NEG_BIG;
+        l[qt] = 0.f;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[qt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    // (the queries have arrived before the first direct load is counted)
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (t0 + wave < t1) stage(t0 + wave, 0);
+    for (int t = t0 + wave, buf = 0; t < t1; t += 4, buf ^= 1) {
+        if (t + 4 < t1) {
+            stage(t + 4, buf ^ 1);
+            asm volatile("s_waitcnt vmcnt(%0)" :: "n"(2 * DMAS) : "memory");
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        const int key0 = tiles.first_key(t, KT);
+        const unsigned char* ks = mine + buf * 2 * I::BYTES;
+        const unsigned char* vs = ks + I::BYTES;
+        f32x4 s[QT][KB];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt) s[qt][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < KC; ++c) {
+                const u32x4 kf = *reinterpret_cast<const u32x4*>(ks + (kb * 16 + r) * I::ROWB + ((4 * c + g) ^ I::k_swizzle(kb * 16 + r)) * 16);
+#pragma unroll
+                for (int qt = 0; qt < QT; ++qt) {
+                    if constexpr (sizeof(E) == 4) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            s[qt][kb] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf[j]), __uint_as_float(qf[qt][c][j]), s[qt][kb], 0, 0, 0);
+                    } else {
+                        s[qt][kb] = MmaFew<E>::mfma(__builtin_bit_cast(typename Mma<E>::x8, kf), __builtin_bit_cast(typename Mma<E>::x8, qf[qt][c]), s[qt][kb]);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) {
+            float mx = NEG_BIG;
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int key = key0 + 16 * kb + 4 * g + i;
+                    const bool ok = key < seen[qt].hi && (key >= seen[qt].lo || key < seen[qt].s);
+                    s[qt][kb][i] = ok ? s[qt][kb][i] : -INFINITY;
+                    mx = fmaxf(mx, s[qt][kb][i]);
+                }
+            mx = quarters_max(mx);
+            if (__any((mx - m[qt]) * scale > LAG)) {
+                const float m_new = fmaxf(m[qt], mx);
+                const float alpha = __builtin_amdgcn_exp2f((m[qt] - m_new) * scale);
+                m[qt] = m_new;
+                l[qt] *= alpha;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[qt][dt][i] *= alpha;
+            }
+            const float ms = m[qt] * scale;
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[qt][kb][i] = __builtin_amdgcn_exp2f(fmaf(s[qt][kb][i], scale, -ms));
+                    l[qt] += s[qt][kb][i];
+                }
+        }
+        if constexpr (sizeof(E) == 4) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int key = 4 * g + i;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                    const float v = *reinterpret_cast<const float*>(vs + key * I::ROWB + (((dt * 4 + (r >> 2)) ^ I::v_swizzle(key)) * 16) + (r & 3) * 4);
+#pragma unroll
+                    for (int qt = 0; qt < QT; ++qt) o[qt][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, s[qt][0][i], o[qt][dt], 0, 0, 0);
+                }
+            }
+        } else {
+            typedef short tr4 __attribute__((__vector_size__(4 * sizeof(short))));
+            typename Mma<E>::x8 pb[QT];
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) pb[qt][j] = (E)s[qt][(j >> 2) % KB][j & 3];
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                union { tr4 t[2]; typename Mma<E>::x8 v; } av;
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int row = 16 * u + 4 * g + (r >> 2);
+                    const unsigned char* p = vs + row * I::ROWB + (((dt * 2 + ((r & 3) >> 1)) ^ I::v_swizzle(row)) * 16) + (r & 1) * 8;
+                    av.t[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) tr4*)p);
+                }
+#pragma unroll
+                for (int qt = 0; qt < QT; ++qt) o[qt][dt] = MmaFew<E>::mfma(av.v, pb[qt], o[qt][dt]);
+            }
+        }
+    }
+
+    // the four waves' results side by side in LDS (each over its own buffers), then one value per thread and step
+    float* sums = reinterpret_cast<float*>(smem);
+    constexpr int WAVE_F = I::BYTES;                          // floats of a wave's buffers: 4 * BYTES / 4
+    static_assert(WAVE_F >= ROWS * D, "a wave's sums fit its buffers");
+    float2* ml = reinterpret_cast<float2*>(smem + 16 * I::BYTES);
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+        const float ls = quarters_sum(l[qt]);
+        if (g == 0) ml[wave * ROWS + 16 * qt + r] = make_float2(m[qt], ls);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(sums + wave * WAVE_F + (16 * qt + r) * D + dt * 16 + 4 * g) = o[qt][dt];
+    }
+    __syncthreads();
+    __shared__ uint32_t bad_rows[2];
+    if (tid < 2) bad_rows[tid] = 0;
+    __syncthreads();
+    for (int i = tid; i < rows * (D / 4); i += 256) {
+        const int lr = i / (D / 4), d = (i % (D / 4)) * 4;
+        const int row = chunk * ROWS + lr, j = row / group, head = kvh * group + row % group;
+        float top = NEG_BIG;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) top = fmaxf(top, ml[w * ROWS + lr].x);
+        float total = 0.f;
+        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float2 p = ml[w * ROWS + lr];
+            const float weight = __builtin_amdgcn_exp2f((p.x - top) * scale);
+            total += p.y * weight;
+            sum += *reinterpret_cast<const f32x4*>(sums + w * WAVE_F + lr * D + d) * weight;
+        }
+        if (f.spans > 1) {
+            const int64_t at = ((sq.q0 + j) * a.hq + head) * (int64_t)f.spans + span;
+            if (d == 0) f.part_ml[at] = make_float2(top, total);
+            *reinterpret_cast<f32x4*>(f.part_o + at * D + d) = sum;
+        } else {
+            const Seen w = seen_by(a, sq.nk - sq.nq + j, sq.nk);
+            const bool any_seen = w.s + (w.hi - w.lo) > 0;
+            const float inv = 1.f / total;
+            typename Vec<E, 4>::type v;
+            bool bad = false;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float x = any_seen ? sum[e] * inv : 0.f;
+                bad |= x != x;
+                v[e] = (E)x;
+            }
+            if (bad) atomicOr(&bad_rows[lr >> 5], 1u << (lr & 31));
+            *reinterpret_cast<typename Vec<E, 4>::type*>(reinterpret_cast<E*>(a.out) + (sq.q0 + j) * a.out_stride + (int64_t)head * D + d) = v;
+        }
+    }
+    if (f.spans > 1) return;
+    __syncthreads();                                         // (also: the rows' stores are done before a row is written again)
+    for (int lr = wave; lr < rows; lr += 4)
+        if (bad_rows[lr >> 5] >> (lr & 31) & 1) {
+            const int row = chunk * ROWS + lr;
+            attend_row<E, D>(a, sq, row / group, kvh * group + row % group, lane);
+        }
+}
+
+// The spans' results of one query row and head, a wave each.
+template <typename E, int D>
+__global__ __launch_bounds__(256) void window_join_kernel(WinArgs a, FewArgs f, int rows_of_chunk, uint32_t* fault) {
+    const int group = a.hq / a.hkv, lane = threadIdx.x & 63;
+    const int per_seq = (a.max_q * a.hq + 3) / 4;
+    const int seq = (int)(blockIdx.x / per_seq);
+    const int id = (int)(blockIdx.x % per_seq) * 4 + (int)(threadIdx.x >> 6);
+    const int j = id / a.hq, head = id % a.hq;
+    Seq sq;
+    if (!load_seq(a, seq, sq, nullptr) || j >= sq.nq) return;
+    const int chunk = (j * group + head % group) / rows_of_chunk;
+    const int last = min((chunk + 1) * rows_of_chunk, sq.nq * group) - 1;
+    const Tiles tiles = tiles_of(a, sq, chunk * rows_of_chunk / group, last / group, FewImage<E, D>::KT);
+    const int n = max(1, (tiles.n + f.span - 1) / f.span);
+    const int64_t at = ((sq.q0 + j) * a.hq + head) * (int64_t)f.spans;
+    const float scale = fabsf(a.scale);
+    float top = NEG_BIG;
+    for (int i = lane; i < n; i += 64) top = fmaxf(top, f.part_ml[at + i].x);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    constexpr int DL = D / 4, PARTS = 64 / DL;               // four dimensions a lane, PARTS spans at a time
+    const int d = (lane % DL) * 4;
+    float total = 0.f;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    for (int i = lane / DL; i < n; i += PARTS) {
+        const float2 p = f.part_ml[at + i];
+        const float weight = __builtin_amdgcn_exp2f((p.x - top) * scale);
+        total += p.y * weight;
+        sum += *reinterpret_cast<const f32x4*>(f.part_o + (at + i) * D + d) * weight;
+    }
+#pragma unroll
+    for (int o = DL; o < 64; o <<= 1) {
+        total += __shfl_xor(total, o, 64);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] += __shfl_xor(sum[e], o, 64);
+    }
+    const Seen w = seen_by(a, sq.nk - sq.nq + j, sq.nk);
+    const bool any_seen = w.s + (w.hi - w.lo) > 0;
+    const float inv = 1.f / total;
+    typename Vec<E, 4>::type v;
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float x = any_seen ? sum[e] * inv : 0.f;
+        bad |= x != x;
+        v[e] = (E)x;
+    }
+    if (__any(bad)) attend_row<E, D>(a, sq, j, head, lane);
+    else if (lane < DL) *reinterpret_cast<typename Vec<E, 4>::type*>(reinterpret_cast<E*>(a.out) + (sq.q0 + j) * a.out_stride + (int64_t)head * D + d) = v;
+}
+
+// How a call runs, from its sizes alone (the workspace is computed from the same).
+struct Plan {
+    bool few;
+    int qt, chunks, spans, span;     // few: 16-row columns of a workgroup, its row chunks, spans along the keys
+    int64_t parts;                   // query rows * heads * spans whose partial results the workspace holds
+};
+Plan plan_of(int64_t total_q, int n_seq, int max_q, int max_k, int hq, int hkv, int D, int left, int right, int sinks, int size) {
+    Plan p{};
+    const int group = hq / hkv;
+    const int64_t rows = (int64_t)max_q * group;
+    p.few = rows <= 64;
+    if (!p.few) return p;
+    p.qt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    p.chunks = (int)((rows + 16 * p.qt - 1) / (16 * p.qt));
+    const int kt = size == 4 ? 16 : 32;
+    // the most keys that the queries of a sequence can see
+    int64_t keys = max_k;
+    if (left >= 0) keys = std::min<int64_t>(keys, (int64_t)sinks + left + max_q + (right < 0 ? max_k : std::min(right, max_k)));
+    const int64_t tiles = std::max<int64_t>(1, (keys + kt - 1) / kt + (left >= 0 ? 2 : 0));
+    const int64_t base = (int64_t)n_seq * hkv * p.chunks;
+    const int64_t want = std::max<int64_t>(1, 768 / base);   // workgroups along the keys that fill the chip three times
+    p.span = (int)std::max<int64_t>(16, (tiles + want - 1) / want);
+    p.spans = (int)((tiles + p.span - 1) / p.span);
+    p.parts = p.spans > 1 ? total_q * hq * p.spans : 0;
+    return p;
+}
+
+template <typename T, int D, int QT>
+int window_few(const WinArgs& a, const Plan& p, void* work, hipStream_t stream) {
+    FewArgs f;
+    f.chunks = p.chunks; f.spans = p.spans; f.span = p.span;
+    f.part_o = reinterpret_cast<float*>(work);
+    f.part_ml = reinterpret_cast<float2*>(f.part_o + p.parts * D);
+    const int64_t grid = (int64_t)a.n_seq * p.spans * p.chunks * a.hkv;
+    RAG_REQUIRE(grid < (1ll << 31), RAG_ELIMIT, "rag_enc_attention_window: too many sequences");
+    constexpr size_t lds = 16 * (size_t)FewImage<T, D>::BYTES + 4 * 16 * QT * sizeof(float2);
+    RAG_GRANT_LDS((window_few_kernel<T, D, QT>), lds);
+    window_few_kernel<T, D, QT><<<(unsigned)grid, 256, lds, stream>>>(a, f, rag_fault_word());
+    RAG_HIP_TRY(hipGetLastError());
+    if (p.spans > 1) {
+        const int64_t joins = (int64_t)a.n_seq * (((int64_t)a.max_q * a.hq + 3) / 4);
+        RAG_REQUIRE(joins < (1ll << 31), RAG_ELIMIT, "rag_enc_attention_window: too many query rows");
+        window_join_kernel<T, D><<<(unsigned)joins, 256, 0, stream>>>(a, f, 16 * QT, rag_fault_word());
+        RAG_HIP_TRY(hipGetLastError());
+    }
+    return RAG_OK;
+}
+
 template <typename T, int D>
-int window_launch(const WinArgs& a, hipStream_t stream) {
+int window_launch(const WinArgs& a, void* work, int64_t work_bytes, hipStream_t stream) {
+    const Plan p = plan_of(a.total_q, a.n_seq, a.max_q, a.max_k, a.hq, a.hkv, D, a.left, a.right, a.sinks, (int)sizeof(T));
+    if (p.few) {
+        RAG_REQUIRE(p.parts * (D + 2) * 4 <= work_bytes, RAG_EINVAL, "rag_enc_attention_window: the workspace holds %lld bytes, %lld are needed",
+                    (long long)work_bytes, (long long)(p.parts * (D + 2) * 4));
+        if (p.qt == 1) return window_few<T, D, 1>(a, p, work, stream);
+        if (p.qt == 2) return window_few<T, D, 2>(a, p, work, stream);
+        return window_few<T, D, 4>(a, p, work, stream);
+    }
     const int q_tiles = (a.max_q + 127) / 128;
     const int64_t units = (int64_t)a.n_seq * q_tiles * a.hq;
     const int64_t grid = (units + 7) / 8 * 8;
@@ -418,20 +822,25 @@ int window_launch(const WinArgs& a, hipStream_t stream) {
 }
 
 template <typename T>
-int window_by_dim(const WinArgs& a, int D, hipStream_t stream) {
-    if (D == 32) return window_launch<T, 32>(a, stream);
-    if (D == 64) return window_launch<T, 64>(a, stream);
-    return window_launch<T, 128>(a, stream);
+int window_by_dim(const WinArgs& a, int D, void* work, int64_t work_bytes, hipStream_t stream) {
+    if (D == 32) return window_launch<T, 32>(a, work, work_bytes, stream);
+    if (D == 64) return window_launch<T, 64>(a, work, work_bytes, stream);
+    return window_launch<T, 128>(a, work, work_bytes, stream);
 }
+
+constexpr int FAR = 1 << 30;         // a window beyond every length is no limit (and positions never overflow)
 
 }  // namespace
 
 extern "C" int64_t rag_enc_attention_window_workspace(int64_t total_q, int32_t n_seq, int32_t max_q_len, int32_t max_k_len,
                                                       int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
-                                                      int32_t window_left, int32_t window_right, int32_t n_sinks) {
-    (void)total_q; (void)n_seq; (void)max_q_len; (void)max_k_len; (void)n_q_heads; (void)n_kv_heads; (void)head_dim;
-    (void)window_left; (void)window_right; (void)n_sinks;
-    return 0;
+                                                      int32_t window_left, int32_t window_right, int32_t n_sinks, int32_t dtype) {
+    if (total_q <= 0 || n_seq <= 0 || max_q_len <= 0 || max_k_len < 0 || n_q_heads <= 0 || n_kv_heads <= 0 || n_q_heads % n_kv_heads || head_dim <= 0 ||
+        n_sinks < 0 || window_left < -1 || window_right < -1)
+        return 0;                                            // nothing to run, or refused by the call
+    const Plan p = plan_of(total_q, n_seq, max_q_len, max_k_len, n_q_heads, n_kv_heads, head_dim, window_left >= FAR ? -1 : window_left,
+                           window_right >= FAR ? -1 : window_right, n_sinks, dtype == RAG_DTYPE_F32 ? 4 : 2);
+    return p.parts * (head_dim + 2) * 4;
 }
 
 extern "C" int rag_enc_attention_window_dev(const void* d_q, int64_t q_stride, const void* d_k, int64_t k_row_stride,
@@ -468,14 +877,13 @@ extern "C" int rag_enc_attention_window_dev(const void* d_q, int64_t q_stride, c
     a.q_stride = q_stride; a.k_row = k_row_stride; a.k_head = k_head_stride; a.v_row = v_row_stride; a.v_head = v_head_stride;
     a.out_stride = out_stride; a.total_q = total_q; a.total_k = total_k;
     a.n_seq = n_seq; a.max_q = max_q_len; a.max_k = d_k_start ? max_k_len : max_q_len; a.hq = n_q_heads; a.hkv = n_kv_heads;
-    const int far = 1 << 30;                                 // beyond every length: no limit, and no overflow
-    a.left = window_left >= far ? -1 : window_left;
-    a.right = window_right >= far ? -1 : window_right;
+    a.left = window_left >= FAR ? -1 : window_left;
+    a.right = window_right >= FAR ? -1 : window_right;
     a.sinks = n_sinks;
     a.scale = scale * 1.4426950408889634f;
-    (void)d_workspace;
+    RAG_REQUIRE(!off(d_workspace) && (d_workspace || workspace_bytes == 0), RAG_EINVAL, "%s: bad workspace", me);
     hipStream_t stream = (hipStream_t)stream_;
-    if (dtype == RAG_DTYPE_F32) return window_by_dim<float>(a, head_dim, stream);
-    if (dtype == RAG_DTYPE_BF16) return window_by_dim<bf16>(a, head_dim, stream);
-    return window_by_dim<f16>(a, head_dim, stream);
+    if (dtype == RAG_DTYPE_F32) return window_by_dim<float>(a, head_dim, d_workspace, workspace_bytes, stream);
+    if (dtype == RAG_DTYPE_BF16) return window_by_dim<bf16>(a, head_dim, d_workspace, workspace_bytes, stream);
+    return window_by_dim<f16>(a, head_dim, d_workspace, workspace_bytes, stream);
 }

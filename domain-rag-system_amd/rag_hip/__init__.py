@@ -107,7 +107,7 @@ SIGNATURES = {
     'rag_enc_linear_ln_split_pack_dev': (_i32, [_vp, _i32, _i32, _vp, _vp, _vp]),
     'rag_enc_qk_norm_rope_dev': (_i32, [_vp, _i64, _vp, _vp, _vp, C.c_float, _vp, _i32, _i32, _i64, _i32, _i32, _i32, _i32, _vp, _i64,
                                         _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp]),
-    'rag_enc_attention_window_workspace': (_i64, [_i64] + [_i32] * 9),
+    'rag_enc_attention_window_workspace': (_i64, [_i64] + [_i32] * 10),
     'rag_enc_attention_window_dev': (_i32, [_vp, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _i32, _i32,
                                             _i32, _i32, _i32, C.c_float, _i32, _i32, _i32, _i32, _vp, _i64, _vp, _i64, _vp]),
     'rag_enc_linear4_dev': (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _i64, _vp]),
@@ -1372,7 +1372,7 @@ def enc_attention_window_dev(q, k, v, cu_q, max_q_len, k_start=None, k_len=None,
     l = lib()
     sizes = (n_seq, int(max_q_len), int(max_k_len), hq, hkv, d)
     window = (int(window_left), int(window_right), int(n_sinks))
-    need = l.rag_enc_attention_window_workspace(tq, *sizes, *window)
+    need = l.rag_enc_attention_window_workspace(tq, *sizes, *window, code)
     work = torch.empty((need,), dtype=torch.uint8, device=q.device) if need > 0 else None
     check(l.rag_enc_attention_window_dev(qp, qs if tq > 1 else hq * d, kp, krs, khs, vp, vrs, vhs, _ptr(cu_q, torch.int32), tq,
                                          _ptr(k_start, torch.int64), _ptr(k_len, torch.int32), tk, *sizes,

@@ -582,7 +582,7 @@ int rag_enc_qk_norm_rope_dev(const void* d_qkv, int64_t qkv_stride, const int32_
  * may be NULL), 16-byte aligned, used by this call alone until it has run on its stream.                    */
 int64_t rag_enc_attention_window_workspace(int64_t total_q, int32_t n_seq, int32_t max_q_len, int32_t max_k_len,
                                            int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
-                                           int32_t window_left, int32_t window_right, int32_t n_sinks);
+                                           int32_t window_left, int32_t window_right, int32_t n_sinks, int32_t dtype);
 int rag_enc_attention_window_dev(const void* d_q, int64_t q_stride, const void* d_k, int64_t k_row_stride,
                                  int64_t k_head_stride, const void* d_v, int64_t v_row_stride, int64_t v_head_stride,
                                  const int32_t* d_cu_q, int64_t total_q, const int64_t* d_k_start,
