@@ -193,20 +193,19 @@ constexpr float LAG = 8.f;           // the maximum may lag behind by this power
 // values hold infinities or NaN, 0 * infinity spoils rows that do not see them: every row that ends as NaN is computed
 // again by attend_row, which reads only what the row sees.
 template <typename E, int D>
-__global__ __launch_bounds__(256, sizeof(E) == 4 ? 1 : 2) void window_tile_kernel(WinArgs a, int q_tiles, int64_t units, uint32_t* fault) {
+__global__ __launch_bounds__(256, sizeof(E) == 4 ? 1 : 2) void window_tile_kernel(WinArgs a, int q_tiles, uint32_t units, uint32_t* fault) {
     typedef Image<E, D> I;
     constexpr int KT = I::KT, KB = KT / 32, DT = D / 32, KC = I::PIECES / 2;
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
     // the units of one (sequence, key/value head) are neighbours, and an eighth of them all goes to each L2
-    const int64_t unit = (int64_t)(blockIdx.x & 7) * ((units + 7) >> 3) + (blockIdx.x >> 3);
-    if ((blockIdx.x >> 3) >= ((units + 7) >> 3) || unit >= units) return;
+    const uint32_t unit = (blockIdx.x & 7) * ((units + 7) >> 3) + (blockIdx.x >> 3);
+    if (unit >= units) return;
     const int group = a.hq / a.hkv;
-    const int g = (int)(unit % group);
-    const int64_t u1 = unit / group;
-    const int qt = q_tiles - 1 - (int)(u1 % q_tiles);        // (a causal sequence's last tiles are its longest)
-    const int64_t u2 = u1 / q_tiles;
-    const int kvh = (int)(u2 % a.hkv), seq = (int)(u2 / a.hkv);
+    const uint32_t u1 = unit / (uint32_t)group, u2 = u1 / (uint32_t)q_tiles;
+    const int g = (int)(unit - u1 * (uint32_t)group);
+    const int qt = q_tiles - 1 - (int)(u1 - u2 * (uint32_t)q_tiles);           // (a causal sequence's last tiles are its longest)
+    const int seq = (int)(u2 / (uint32_t)a.hkv), kvh = (int)(u2 - (uint32_t)seq * (uint32_t)a.hkv);
     const int head = kvh * group + g;
     Seq sq;
     if (!load_seq(a, seq, sq, fault) || qt * 128 >= sq.nq) return;
@@ -410,8 +409,8 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 ? 1 : 2) void window_tile_kerne
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // The rows of one key/value head's queries (row = query * group + head of the group) are the columns of the matrix
-// products, 16 * QT of them per workgroup, so that a key is read once for all of them.  Four waves take tiles of keys in turn,
-// each into its own two LDS buffers (no barrier until the end), and put their results together; a long text is cut
+// products, 16 * QT of them per workgroup, so that a key is read once for all of them.  Its waves take tiles of keys in
+// turn, each into its own two LDS buffers (no barrier until the end), and put their results together; a long text is cut
 // into spans of `span` tiles, one workgroup each, whose results window_join_kernel puts together.
 // Bound by the bytes of the keys and values: 64 KB of loads are in flight per compute unit.
 template <typename E, int D> struct FewImage {
@@ -419,6 +418,8 @@ template <typename E, int D> struct FewImage {
     static constexpr int PIECES = ROWB / 16;
     static constexpr int KT = sizeof(E) == 4 ? 16 : 32;      // keys of a wave's tile
     static constexpr int BYTES = KT * ROWB;
+    static constexpr int NW = 4;                             // waves
+    static constexpr size_t lds(int rows) { return (size_t)NW * (4 * BYTES + rows * 8); }
     __device__ static int k_swizzle(int row) { return Image<E, D>::k_swizzle(row); }
     // 16 bits: 8 neighbouring rows x 2 neighbouring pieces; 32 bits: rows 4 apart, 4 pieces
     __device__ static int v_swizzle(int row) {
@@ -470,18 +471,15 @@ struct FewArgs {
 };
 
 template <typename E, int D, int QT>
-__global__ __launch_bounds__(256) void window_few_kernel(WinArgs a, FewArgs f, uint32_t* fault) {
+__global__ __launch_bounds__(64 * (FewImage<E, D>::NW)) void window_few_kernel(WinArgs a, FewArgs f, uint32_t* fault) {
     typedef FewImage<E, D> I;
-    constexpr int KT = I::KT, KB = KT / 16, DT = D / 16, KC = I::PIECES / 4, ROWS = 16 * QT;
+    constexpr int KT = I::KT, KB = KT / 16, DT = D / 16, KC = I::PIECES / 4, ROWS = 16 * QT, NW = I::NW;
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-    extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];       // [4 waves][2 buffers][K | V], later [4][ROWS][D] sums; [4][ROWS] (m, l)
+    extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];       // [waves][2 buffers][K | V], later [waves][ROWS][D] sums; [waves][ROWS] (m, l)
     const int group = a.hq / a.hkv;
-    const int64_t unit = blockIdx.x;
-    const int kvh = (int)(unit % a.hkv);
-    const int64_t u1 = unit / a.hkv;
-    const int chunk = (int)(u1 % f.chunks);
-    const int64_t u2 = u1 / f.chunks;
-    const int span = (int)(u2 % f.spans), seq = (int)(u2 / f.spans);
+    const uint32_t u1 = blockIdx.x / (uint32_t)a.hkv, u2 = u1 / (uint32_t)f.chunks;
+    const int kvh = (int)(blockIdx.x - u1 * (uint32_t)a.hkv), chunk = (int)(u1 - u2 * (uint32_t)f.chunks);
+    const int seq = (int)(u2 / (uint32_t)f.spans), span = (int)(u2 - (uint32_t)seq * (uint32_t)f.spans);
     Seq sq;
     if (!load_seq(a, seq, sq, fault)) return;
     const int rows = min(ROWS, sq.nq * group - chunk * ROWS);
@@ -519,6 +517,7 @@ __global__ __launch_bounds__(256) void window_few_kernel(WinArgs a, FewArgs f, u
         }
     };
 
+    if (t0 + wave < t1) stage(t0 + wave, 0);
     const bool flip = a.scale < 0.f;
     const float scale = fabsf(a.scale);
     u32x4 qf[QT][KC];
@@ -543,12 +542,14 @@ __global__ __launch_bounds__(256) void window_few_kernel(WinArgs a, FewArgs f, u
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) o[qt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    // (the queries have arrived before the first direct load is counted)
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if (t0 + wave < t1) stage(t0 + wave, 0);
-    for (int t = t0 + wave, buf = 0; t < t1; t += 4, buf ^= 1) {
-        if (t + 4 < t1) {
-            stage(t + 4, buf ^ 1);
+    // (the queries, the last loads so far, are waited for here: inside the loop their wait would cover the next tile too)
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+        for (int c = 0; c < KC; ++c) asm volatile("" : "+v"(qf[qt][c]));
+    for (int t = t0 + wave, buf = 0; t < t1; t += NW, buf ^= 1) {
+        if (t + NW < t1) {
+            stage(t + NW, buf ^ 1);
             asm volatile("s_waitcnt vmcnt(%0)" :: "n"(2 * DMAS) : "memory");
         } else {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -641,11 +642,11 @@ __global__ __launch_bounds__(256) void window_few_kernel(WinArgs a, FewArgs f, u
         }
     }
 
-    // the four waves' results side by side in LDS (each over its own buffers), then one value per thread and step
+    // the waves' results side by side in LDS (each over its own buffers), then one value per thread and step
     float* sums = reinterpret_cast<float*>(smem);
     constexpr int WAVE_F = I::BYTES;                          // floats of a wave's buffers: 4 * BYTES / 4
     static_assert(WAVE_F >= ROWS * D, "a wave's sums fit its buffers");
-    float2* ml = reinterpret_cast<float2*>(smem + 16 * I::BYTES);
+    float2* ml = reinterpret_cast<float2*>(smem + NW * 4 * I::BYTES);
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
         const float ls = quarters_sum(l[qt]);
@@ -657,16 +658,16 @@ __global__ __launch_bounds__(256) void window_few_kernel(WinArgs a, FewArgs f, u
     __shared__ uint32_t bad_rows[2];
     if (tid < 2) bad_rows[tid] = 0;
     __syncthreads();
-    for (int i = tid; i < rows * (D / 4); i += 256) {
+    for (int i = tid; i < rows * (D / 4); i += 64 * NW) {
         const int lr = i / (D / 4), d = (i % (D / 4)) * 4;
         const int row = chunk * ROWS + lr, j = row / group, head = kvh * group + row % group;
         float top = NEG_BIG;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) top = fmaxf(top, ml[w * ROWS + lr].x);
+        for (int w = 0; w < NW; ++w) top = fmaxf(top, ml[w * ROWS + lr].x);
         float total = 0.f;
         f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < NW; ++w) {
             const float2 p = ml[w * ROWS + lr];
             const float weight = __builtin_amdgcn_exp2f((p.x - top) * scale);
             total += p.y * weight;
@@ -694,7 +695,7 @@ __global__ __launch_bounds__(256) void window_few_kernel(WinArgs a, FewArgs f, u
     }
     if (f.spans > 1) return;
     __syncthreads();                                         // (also: the rows' stores are done before a row is written again)
-    for (int lr = wave; lr < rows; lr += 4)
+    for (int lr = wave; lr < rows; lr += NW)
         if (bad_rows[lr >> 5] >> (lr & 31) & 1) {
             const int row = chunk * ROWS + lr;
             attend_row<E, D>(a, sq, row / group, kvh * group + row % group, lane);
@@ -772,8 +773,15 @@ Plan plan_of(int64_t total_q, int n_seq, int max_q, int max_k, int hq, int hkv, 
     if (left >= 0) keys = std::min<int64_t>(keys, (int64_t)sinks + left + max_q + (right < 0 ? max_k : std::min(right, max_k)));
     const int64_t tiles = std::max<int64_t>(1, (keys + kt - 1) / kt + (left >= 0 ? 2 : 0));
     const int64_t base = (int64_t)n_seq * hkv * p.chunks;
-    const int64_t want = std::max<int64_t>(1, 768 / base);   // workgroups along the keys that fill the chip three times
-    p.span = (int)std::max<int64_t>(16, (tiles + want - 1) / want);
+    // A workgroup's start, the filling of its buffers and its end cost as much as some 8 tiles a wave, so the workgroups that are on
+    // the chip at once (256 compute units by what their LDS leaves room for) run one round: one token over 32768 keys of 8 heads
+    // 36.6 us, in two rounds 44, in three 51.  Spans that would be long all the same (over 256 tiles) are cut in three, against
+    // sequences of unlike lengths: 16 sequences of 4000 to 32768 keys 223 -> 190 us.  Below 8 tiles a span, or 20 in all,
+    // joining costs more than it gives (window 1024: spans of 16 tiles 11.5 us, 8: 10.0; 512 keys: one span 8.2 us, two 9.3).
+    const int64_t on_chip = 256 * ((160 << 10) / (16 * (int64_t)kt * D * size + 2048));
+    int64_t cuts = std::max<int64_t>(1, on_chip / base);
+    if (tiles / cuts > 256) cuts = std::max<int64_t>(1, 3 * on_chip / base);
+    p.span = (int)(tiles <= 20 ? tiles : std::max<int64_t>(8, (tiles + cuts - 1) / cuts));
     p.spans = (int)((tiles + p.span - 1) / p.span);
     p.parts = p.spans > 1 ? total_q * hq * p.spans : 0;
     return p;
@@ -787,9 +795,9 @@ int window_few(const WinArgs& a, const Plan& p, void* work, hipStream_t stream) 
     f.part_ml = reinterpret_cast<float2*>(f.part_o + p.parts * D);
     const int64_t grid = (int64_t)a.n_seq * p.spans * p.chunks * a.hkv;
     RAG_REQUIRE(grid < (1ll << 31), RAG_ELIMIT, "rag_enc_attention_window: too many sequences");
-    constexpr size_t lds = 16 * (size_t)FewImage<T, D>::BYTES + 4 * 16 * QT * sizeof(float2);
+    constexpr size_t lds = FewImage<T, D>::lds(16 * QT);
     RAG_GRANT_LDS((window_few_kernel<T, D, QT>), lds);
-    window_few_kernel<T, D, QT><<<(unsigned)grid, 256, lds, stream>>>(a, f, rag_fault_word());
+    window_few_kernel<T, D, QT><<<(unsigned)grid, 64 * FewImage<T, D>::NW, lds, stream>>>(a, f, rag_fault_word());
     RAG_HIP_TRY(hipGetLastError());
     if (p.spans > 1) {
         const int64_t joins = (int64_t)a.n_seq * (((int64_t)a.max_q * a.hq + 3) / 4);
@@ -816,7 +824,7 @@ int window_launch(const WinArgs& a, void* work, int64_t work_bytes, hipStream_t 
     RAG_REQUIRE(grid < (1ll << 31), RAG_ELIMIT, "rag_enc_attention_window: too many query tiles");
     constexpr size_t lds = 4 * (size_t)Image<T, D>::BYTES;
     RAG_GRANT_LDS((window_tile_kernel<T, D>), lds);
-    window_tile_kernel<T, D><<<(unsigned)grid, 256, lds, stream>>>(a, q_tiles, units, rag_fault_word());
+    window_tile_kernel<T, D><<<(unsigned)grid, 256, lds, stream>>>(a, q_tiles, (uint32_t)units, rag_fault_word());
     RAG_HIP_TRY(hipGetLastError());
     return RAG_OK;
 }

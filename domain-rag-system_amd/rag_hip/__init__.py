@@ -4,6 +4,7 @@ The library is the only compute backend of this package: when it is missing, or 
 gfx950 GPU is usable, the entry points raise.  There is no CPU fallback.
 """
 import ctypes as C
+import functools
 import os
 import threading
 
@@ -1245,30 +1246,49 @@ def enc_linear_ln_split_profile_read():
 
 
 # ---- encoders with rotary positions, windowed layers, 4-bit weights ---------------------------------
+# One token's call takes the GPU a few microseconds, so what the host does around it counts: these wrappers ask for the
+# device and the stream once and for every tensor's facts once.
+_ENC_CODES = {}
+
+
 def _enc_code(dtype):
-    import torch
-    code = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16}.get(dtype)
+    if not _ENC_CODES:
+        import torch
+        _ENC_CODES.update({torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16})
+    code = _ENC_CODES.get(dtype)
     if code is None:
         raise ValueError(f"the encoder kernels handle float32, bfloat16 and float16, not {dtype}")
     return code
 
 
-def _same_device(*tensors):
-    """Every tensor given (None: skipped) is on the current GPU, whose stream the kernels are launched on."""
+def _here_and_stream(*tensors):
+    """The current stream of the current GPU, after checking that every tensor given (None: skipped) is on that GPU."""
     import torch
     here = torch.cuda.current_device()
     for t in tensors:
         if t is not None and t.get_device() != here:
             raise ValueError(f"rag_hip launches on the current GPU (cuda:{here}); a tensor is on {t.device}")
+    raw = getattr(torch._C, '_cuda_getCurrentRawStream', None)      # (current_stream() builds an object around it: 4 us)
+    return raw(here) if raw is not None else torch.cuda.current_stream(here).cuda_stream
+
+
+def _flat(t, dtype, name):
+    """Pointer of a contiguous tensor of that type (None: NULL)."""
+    if t is None:
+        return None
+    if t.dtype != dtype or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor")
+    return t.data_ptr()
 
 
 def _heads_view(t, dtype, name):
     """(pointer, row stride, head stride) of a [rows, heads, head_dim] tensor whose head rows are contiguous."""
-    if t.dim() != 3 or t.dtype != dtype:
-        raise ValueError(f"{name} must be a {dtype} tensor [rows, heads, head_dim]")
-    if t.shape[2] != 1 and t.stride(2) != 1:
+    if t.dtype != dtype:
+        raise ValueError(f"{name} must be a {dtype} tensor")
+    row, head, one = t.stride()
+    if one != 1:
         raise ValueError(f"the dimensions of a head of {name} must be contiguous")
-    return t.data_ptr(), t.stride(0), t.stride(1)
+    return t.data_ptr(), row, head
 
 
 def rope_inv_freq(rot_dim, theta=10000.0, device='cuda'):
@@ -1286,43 +1306,42 @@ def enc_qk_norm_rope_dev(qkv, pos, inv_freq, n_q_heads, n_kv_heads, gamma_q=None
     [rows, n_kv_heads, D] (kept keys and values) token t's go to row kv_row[t] (int64 [T], distinct; < 0: nowhere; None:
     row t) of those."""
     import torch
-    if qkv.dim() != 2 or not qkv.is_cuda or (qkv.shape[1] > 1 and qkv.stride(1) != 1):
+    if qkv.dim() != 2 or not qkv.is_cuda or qkv.stride(1) != 1:
         raise ValueError("qkv must be a 2-d GPU tensor with contiguous rows")
-    dt, t, heads = qkv.dtype, qkv.shape[0], n_q_heads + 2 * n_kv_heads
+    dt, (t, width), heads = qkv.dtype, qkv.shape, n_q_heads + 2 * n_kv_heads
     code = _enc_code(dt)
-    if n_q_heads < 1 or n_kv_heads < 1 or qkv.shape[1] % heads:
+    if n_q_heads < 1 or n_kv_heads < 1 or width % heads:
         raise ValueError("a row of qkv must hold n_q_heads + 2 n_kv_heads heads")
-    d = qkv.shape[1] // heads
-    rot = 2 * inv_freq.shape[0] if inv_freq is not None else 0
-    if pos is not None and tuple(pos.shape) != (t,):
+    d = width // heads
+    rot = 2 * inv_freq.numel() if inv_freq is not None else 0
+    if pos is not None and pos.shape != (t,):
         raise ValueError("pos must have one entry per token")
-    for g in (gamma_q, gamma_k):
-        if g is not None and tuple(g.shape) != (d,):
-            raise ValueError("gamma_q and gamma_k must have one entry per dimension of a head")
-    if (v_out is not None and k_out is None) or (kv_row is not None and k_out is None):
+    if (gamma_q is not None and gamma_q.shape != (d,)) or (gamma_k is not None and gamma_k.shape != (d,)):
+        raise ValueError("gamma_q and gamma_k must have one entry per dimension of a head")
+    if k_out is None and (v_out is not None or kv_row is not None):
         raise ValueError("v_out and kv_row need k_out")
-    if kv_row is not None and tuple(kv_row.shape) != (t,):
+    if kv_row is not None and kv_row.shape != (t,):
         raise ValueError("kv_row must have one entry per token")
     if q_out is None:
         q_out = torch.empty((t, n_q_heads, d), dtype=dt, device=qkv.device)
-    elif tuple(q_out.shape) != (t, n_q_heads, d) or (n_q_heads > 1 and q_out.stride(1) != d):
+    elif q_out.shape != (t, n_q_heads, d) or (n_q_heads > 1 and q_out.stride(1) != d):
         raise ValueError("q_out must be [T, n_q_heads, D] with the heads of a row side by side")
     if k_out is None:
         k_out = torch.empty((t, n_kv_heads, d), dtype=dt, device=qkv.device)
-    for name, o in (('k_out', k_out), ('v_out', v_out)):
-        if o is not None and (o.dim() != 3 or tuple(o.shape[1:]) != (n_kv_heads, d) or (kv_row is None and o.shape[0] < t)):
-            raise ValueError(f"{name} must be [rows, n_kv_heads, D] with a row for every token")
-    if v_out is not None and v_out.shape[0] != k_out.shape[0]:
-        raise ValueError("k_out and v_out must have the same rows")
-    _same_device(qkv, pos, inv_freq, gamma_q, gamma_k, q_out, k_out, v_out, kv_row)
+    rows = k_out.shape[0]
+    if k_out.shape != (rows, n_kv_heads, d) or (kv_row is None and rows < t):
+        raise ValueError("k_out must be [rows, n_kv_heads, D] with a row for every token")
+    if v_out is not None and v_out.shape != k_out.shape:
+        raise ValueError("v_out must have the shape of k_out")
+    stream = _here_and_stream(qkv, pos, inv_freq, gamma_q, gamma_k, q_out, k_out, v_out, kv_row)
     qp, qs, _ = _heads_view(q_out, dt, 'q_out')
     kp, krs, khs = _heads_view(k_out, dt, 'k_out')
     vp, vrs, vhs = _heads_view(v_out, dt, 'v_out') if v_out is not None else (None, 0, 0)
-    stride = qkv.stride(0) if t > 1 else qkv.shape[1]
-    check(lib().rag_enc_qk_norm_rope_dev(qkv.data_ptr(), stride, _ptr(pos, torch.int32), _ptr(gamma_q, dt), _ptr(gamma_k, dt), float(eps),
-                                         _ptr(inv_freq, torch.float64), rot, 1 if interleaved else 0, t, n_q_heads, n_kv_heads, d,
-                                         code, qp, qs if t > 1 else n_q_heads * d, kp, krs, khs, vp, vrs, vhs, _ptr(kv_row, torch.int64),
-                                         k_out.shape[0], _stream()), 'rag_enc_qk_norm_rope_dev')
+    check(lib().rag_enc_qk_norm_rope_dev(qkv.data_ptr(), qkv.stride(0) if t > 1 else width, _flat(pos, torch.int32, 'pos'),
+                                         _flat(gamma_q, dt, 'gamma_q'), _flat(gamma_k, dt, 'gamma_k'), eps,
+                                         _flat(inv_freq, torch.float64, 'inv_freq'), rot, 1 if interleaved else 0, t, n_q_heads,
+                                         n_kv_heads, d, code, qp, qs if t > 1 else n_q_heads * d, kp, krs, khs, vp, vrs, vhs,
+                                         _flat(kv_row, torch.int64, 'kv_row'), rows, stream), 'rag_enc_qk_norm_rope_dev')
     if v_out is None:
         v_out = qkv.unflatten(1, (heads, d))[:, n_q_heads + n_kv_heads:]
     return q_out, k_out, v_out
@@ -1340,46 +1359,50 @@ def enc_attention_window_dev(q, k, v, cu_q, max_q_len, k_start=None, k_len=None,
     import torch
     dt = q.dtype
     code = _enc_code(dt)
-    if not q.is_cuda or q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3 or not q.is_cuda:
         raise ValueError("q, k and v must be GPU tensors [rows, heads, head_dim]")
     tq, hq, d = q.shape
-    tk, hkv, _ = k.shape
-    if k.shape != v.shape or k.shape[2] != d or hkv < 1 or hq < 1 or hq % hkv:
+    tk, hkv, dk = k.shape
+    if k.shape != v.shape or dk != d or hkv < 1 or hq < 1 or hq % hkv:
         raise ValueError("k and v must have the same shape, the head size of q, and a divisor of its heads")
-    if (k_start is None) != (k_len is None):
-        raise ValueError("k_start and k_len come together")
-    n_seq = cu_q.shape[0] - 1
-    if n_seq < 0 or cu_q.dim() != 1:
+    if cu_q.dim() != 1 or cu_q.shape[0] < 1:
         raise ValueError("cu_q must have one entry more than there are sequences")
+    n_seq = cu_q.shape[0] - 1
     if k_start is None:
+        if k_len is not None:
+            raise ValueError("k_start and k_len come together")
         if tk != tq:
             raise ValueError("without k_start, k and v must have the rows of q")
         max_k_len = max_q_len
-    elif tuple(k_start.shape) != (n_seq,) or tuple(k_len.shape) != (n_seq,):
+    elif k_len is None or max_k_len is None:
+        raise ValueError("kept keys need k_start, k_len and max_k_len, the longest of k_len")
+    elif k_start.shape != (n_seq,) or k_len.shape != (n_seq,):
         raise ValueError("k_start and k_len must have one entry per sequence")
-    elif max_k_len is None:
-        raise ValueError("kept keys need max_k_len, the longest of k_len")
     if out is None:
         out = torch.empty((tq, hq * d), dtype=dt, device=q.device)
-    elif tuple(out.shape) != (tq, hq * d) or out.dtype != dt or (tq > 0 and out.stride(1) != 1):
+    elif out.shape != (tq, hq * d) or out.dtype != dt or out.stride(1) != 1:
         raise ValueError("out must be [Tq, Hq * D] of q's type with contiguous rows")
-    _same_device(q, k, v, cu_q, k_start, k_len, out)
-    if hq > 1 and q.stride(1) != d:
-        raise ValueError("the heads of a row of q must lie side by side")
-    qp, qs, _ = _heads_view(q, dt, 'q')
+    stream = _here_and_stream(q, k, v, cu_q, k_start, k_len, out)
+    qp, qs, qhs = _heads_view(q, dt, 'q')
     kp, krs, khs = _heads_view(k, dt, 'k')
     vp, vrs, vhs = _heads_view(v, dt, 'v')
-    l = lib()
-    sizes = (n_seq, int(max_q_len), int(max_k_len), hq, hkv, d)
-    window = (int(window_left), int(window_right), int(n_sinks))
-    need = l.rag_enc_attention_window_workspace(tq, *sizes, *window, code)
+    if hq > 1 and qhs != d:
+        raise ValueError("the heads of a row of q must lie side by side")
+    max_q_len, max_k_len, window_left, window_right, n_sinks = int(max_q_len), int(max_k_len), int(window_left), int(window_right), int(n_sinks)
+    need = _window_workspace(tq, n_seq, max_q_len, max_k_len, hq, hkv, d, window_left, window_right, n_sinks, code)
     work = torch.empty((need,), dtype=torch.uint8, device=q.device) if need > 0 else None
-    check(l.rag_enc_attention_window_dev(qp, qs if tq > 1 else hq * d, kp, krs, khs, vp, vrs, vhs, _ptr(cu_q, torch.int32), tq,
-                                         _ptr(k_start, torch.int64), _ptr(k_len, torch.int32), tk, *sizes,
-                                         float(d ** -0.5 if scale is None else scale), *window, code, out.data_ptr(),
-                                         out.stride(0) if tq > 1 else hq * d, _ptr(work), max(need, 0), _stream()),
-          'rag_enc_attention_window_dev')
+    check(lib().rag_enc_attention_window_dev(qp, qs if tq > 1 else hq * d, kp, krs, khs, vp, vrs, vhs, _flat(cu_q, torch.int32, 'cu_q'), tq,
+                                             _flat(k_start, torch.int64, 'k_start'), _flat(k_len, torch.int32, 'k_len'), tk, n_seq,
+                                             max_q_len, max_k_len, hq, hkv, d, d ** -0.5 if scale is None else scale, window_left,
+                                             window_right, n_sinks, code, out.data_ptr(), out.stride(0) if tq > 1 else hq * d,
+                                             work.data_ptr() if work is not None else None, need, stream), 'rag_enc_attention_window_dev')
     return out
+
+
+@functools.lru_cache(maxsize=4096)
+def _window_workspace(*sizes):
+    """rag_enc_attention_window_workspace, which goes by the sizes alone."""
+    return load_library().rag_enc_attention_window_workspace(*sizes)
 
 
 def quantize4(weight, group=64, dtype=None, symmetric=False):
@@ -1414,22 +1437,21 @@ def enc_linear4_dev(x, codes, scales, offsets=None, bias=None, out=None):
     import torch
     dt = x.dtype
     code = _enc_code(dt)
-    if x.dim() != 2 or not x.is_cuda or (x.shape[1] > 1 and x.stride(1) != 1):
-        raise ValueError("x must be a 2-d GPU tensor with contiguous rows")
-    m, k = x.shape
-    n = codes.shape[0]
-    if codes.dim() != 2 or codes.shape[1] * 2 != k or scales.dim() != 2 or scales.shape[0] != n or scales.shape[1] < 1 or k % scales.shape[1]:
+    if x.dim() != 2 or codes.dim() != 2 or scales.dim() != 2 or not x.is_cuda or x.stride(1) != 1:
+        raise ValueError("x must be a 2-d GPU tensor with contiguous rows, codes and scales 2-d")
+    (m, k), (n, half), (sn, groups) = x.shape, codes.shape, scales.shape
+    if half * 2 != k or sn != n or groups < 1 or k % groups:
         raise ValueError("codes must be [N, K / 2] and scales [N, K / group]")
     if offsets is not None and offsets.shape != scales.shape:
         raise ValueError("offsets must have the shape of scales")
-    if bias is not None and tuple(bias.shape) != (n,):
+    if bias is not None and bias.shape != (n,):
         raise ValueError("bias must have one entry per row of the weights")
     if out is None:
         out = torch.empty((m, n), dtype=dt, device=x.device)
-    elif tuple(out.shape) != (m, n) or out.dtype != dt or (n > 1 and out.stride(1) != 1):
+    elif out.shape != (m, n) or out.dtype != dt or out.stride(1) != 1:
         raise ValueError("out must be [M, N] of x's type with contiguous rows")
-    _same_device(x, codes, scales, offsets, bias, out)
-    check(lib().rag_enc_linear4_dev(x.data_ptr(), x.stride(0) if m > 1 else k, _ptr(codes, torch.uint8), _ptr(scales, dt), _ptr(offsets, dt),
-                                    _ptr(bias, dt), m, n, k, k // scales.shape[1], code, out.data_ptr(),
-                                    out.stride(0) if m > 1 else n, _stream()), 'rag_enc_linear4_dev')
+    stream = _here_and_stream(x, codes, scales, offsets, bias, out)
+    check(lib().rag_enc_linear4_dev(x.data_ptr(), x.stride(0) if m > 1 else k, _flat(codes, torch.uint8, 'codes'), _flat(scales, dt, 'scales'),
+                                    _flat(offsets, dt, 'offsets'), _flat(bias, dt, 'bias'), m, n, k, k // groups, code, out.data_ptr(),
+                                    out.stride(0) if m > 1 else n, stream), 'rag_enc_linear4_dev')
     return out
