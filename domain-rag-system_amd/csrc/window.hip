@@ -156,6 +156,9 @@ template <typename E, int D> struct Image {
     static constexpr int PIECES = ROWB / 16;
     static constexpr int KT = sizeof(E) == 4 ? 32 : 64;      // keys of a tile
     static constexpr int BYTES = KT * ROWB;
+    // tiles in LDS at a time: what the registers' occupancy leaves room for
+    static constexpr int BUFFERS = BYTES > 4096 ? 2 : 4;
+    static constexpr int WAVES = sizeof(E) == 4 ? (D == 128 ? 1 : D == 64 ? 2 : 4) : (D == 128 ? 2 : D == 64 ? 3 : 4);        // per SIMD
     // 16 neighbouring rows at one piece index cover all banks once
     __device__ static int k_swizzle(int row) {
         return PIECES >= 16 ? row & 15 : PIECES == 8 ? (row >> 1) & 7 : (row >> 2) & 3;
@@ -177,11 +180,14 @@ template <> struct Mma<f16> {
     __device__ static f32x16 mfma(x8 a, x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 };
 
+// the lowest n bits (none for n <= 0, all for n >= 32)
+__device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
+
 constexpr float NEG_BIG = -1e30f;    // the running maximum's start: finite, so that no difference of infinities arises
 constexpr float LAG = 8.f;           // the maximum may lag behind by this power of two before the sums are rescaled
 
 // Four waves, each 32 queries (the columns of the matrix products) of a 128-query tile of one head; tiles of keys and values
-// come into LDS by direct loads, two buffers, the next tile's loads in flight while this one is worked on, one barrier a tile.
+// come into LDS by direct loads into a ring of two to four, the next tiles' loads in flight while this one is worked on, one barrier a tile.
 //   S^T = K Q^T        rows = keys, a lane holds 16 keys (registers, lane half) of its query (lane % 32)
 //   O^T += V^T P^T     the lane's probabilities are the B operand as they stand; V^T comes out of the row-major image
 //                      through the transposing LDS read (16 bits) or by single values (fp32)
@@ -189,17 +195,25 @@ constexpr float LAG = 8.f;           // the maximum may lag behind by this power
 // sums.  fp32: v_mfma_f32_32x32x2_f32, exact fp32 products.
 // The running maximum is only raised when a score exceeds it by 2^LAG (the probabilities then stay below 2^LAG, exact in
 // every type), so that the rescaling of the sums is rare.
-// Masked scores are -infinity; a tile that every query of the wave sees whole needs no mask.  Where keys or
+// Masked scores are -infinity; a tile that every query of the wave sees whole needs no mask, one that none
+// sees is left out.  Where keys or
 // values hold infinities or NaN, 0 * infinity spoils rows that do not see them: every row that ends as NaN is computed
 // again by attend_row, which reads only what the row sees.
 template <typename E, int D>
-__global__ __launch_bounds__(256, sizeof(E) == 4 ? 1 : 2) void window_tile_kernel(WinArgs a, int q_tiles, uint32_t units, uint32_t* fault) {
+__global__ __launch_bounds__(256, (Image<E, D>::WAVES)) void window_tile_kernel(WinArgs a, int q_tiles, uint32_t units, bool by_pair, uint32_t* fault) {
     typedef Image<E, D> I;
-    constexpr int KT = I::KT, KB = KT / 32, DT = D / 32, KC = I::PIECES / 2;
+    constexpr int KT = I::KT, KB = KT / 32, DT = D / 32, KC = I::PIECES / 2, NB = I::BUFFERS;
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-    // the units of one (sequence, key/value head) are neighbours, and an eighth of them all goes to each L2
-    const uint32_t unit = (blockIdx.x & 7) * ((units + 7) >> 3) + (blockIdx.x >> 3);
+    // All units of a (sequence, key/value head) pair go to workgroups with the same blockIdx % 8, which round-robin
+    // placement puts on one XCD: its L2 then holds their keys and values.  Fewer pairs than fill the XCDs evenly: an eighth of
+    // the units, neighbours, goes to each instead.
+    const uint32_t xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
+    uint32_t unit = xcd * ((units + 7) >> 3) + at;
+    if (by_pair) {
+        const uint32_t per_pair = (uint32_t)(a.hq / a.hkv) * (uint32_t)q_tiles, turn = at / per_pair;
+        unit = (turn * 8 + xcd) * per_pair + (at - turn * per_pair);
+    }
     if (unit >= units) return;
     const int group = a.hq / a.hkv;
     const uint32_t u1 = unit / (uint32_t)group, u2 = u1 / (uint32_t)q_tiles;
@@ -234,7 +248,7 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 ? 1 : 2) void window_tile_kerne
         const int key0 = first_key(t);
         const int last = sq.nk - 1 - key0;                   // rows beyond the last key repeat it (masked)
         const unsigned char *kp = kbase + (int64_t)key0 * k_rowb, *vp = vbase + (int64_t)key0 * v_rowb;
-        const uint32_t dst = lds0 + (t & 1) * 2 * I::BYTES;
+        const uint32_t dst = lds0 + (t % NB) * 2 * I::BYTES;
 #pragma unroll
         for (int j = 0; j < I::BYTES / 4096; ++j) {
             const int n = wave + 4 * j, o = n * 1024 + lane * 16;
@@ -258,6 +272,12 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 ? 1 : 2) void window_tile_kerne
             if (flip) qf[c] ^= sizeof(E) == 4 ? 0x80000000u : 0x80008000u;
         }
     }
+    // (the queries, the last loads so far, are waited for here: later their wait would cover the tiles behind the first too)
+#pragma unroll
+    for (int c = 0; c < KC; ++c) asm volatile("" : "+v"(qf[c]));
+#pragma unroll
+    for (int t = 1; t < NB - 1; ++t)
+        if (t < n_tiles) stage(t);
     float m_run = NEG_BIG, l_run = 0.f;                      // l_run: the lane's own keys
     f32x16 o[DT];
 #pragma unroll
@@ -266,19 +286,26 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 ? 1 : 2) void window_tile_kerne
         for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
 
     for (int t = 0; t < n_tiles; ++t) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // this tile's loads
-        __syncthreads();
-        if (t + 1 < n_tiles) stage(t + 1);
+        // this tile's loads; those of the next NB - 2 stay in flight
+        if (NB > 2 && t + NB - 2 < n_tiles) asm volatile("s_waitcnt vmcnt(%0)" :: "n"((NB - 2) * (I::BYTES / 2048)) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();                        // every wave has its part, and is done with the tile before
+        asm volatile("" ::: "memory");
+        if (t + NB - 1 < n_tiles) stage(t + NB - 1);
         const int key0 = first_key(t);
+        // whether some query of the wave sees some of the tile, and whether all see all of it
         const bool some = wave_on && key0 < w_last.hi && (key0 + KT > w_first.lo || key0 < a.sinks);
         if (!some) continue;
-        const unsigned char* ks = smem + (t & 1) * 2 * I::BYTES;
+        const bool whole = key0 + KT <= w_first.hi && (key0 >= w_last.lo || key0 + KT <= a.sinks);
+        const unsigned char* ks = smem + (t % NB) * 2 * I::BYTES;
         const unsigned char* vs = ks + I::BYTES;
         f32x16 s[KB];
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
+        for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[kb][i] = 0.f;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
             for (int c = 0; c < KC; ++c) {
                 const u32x4 kf = *reinterpret_cast<const u32x4*>(ks + (kb * 32 + r) * I::ROWB + ((2 * c + h) ^ I::k_swizzle(r)) * 16);
@@ -291,16 +318,18 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 ? 1 : 2) void window_tile_kerne
                 }
             }
         }
-        const bool whole = key0 + KT <= w_first.hi && (key0 >= w_last.lo || key0 + KT <= a.sinks);
         if (!whole) {
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
+            for (int kb = 0; kb < KB; ++kb) {
+                // a bit per key of the block: [lo, hi) and [0, s)
+                const int k0 = key0 + 32 * kb;
+                const uint32_t seen = ((below(mine.hi - k0) & ~below(mine.lo - k0)) | below(mine.s - k0)) >> (4 * h);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const int key = key0 + 32 * kb + 8 * (i >> 2) + 4 * h + (i & 3);
-                    const bool seen = key < mine.hi && (key >= mine.lo || key < mine.s);
-                    s[kb][i] = seen ? s[kb][i] : -INFINITY;
+                    const uint32_t keep = (uint32_t)((int32_t)(seen << (31 - (8 * (i >> 2) + (i & 3)))) >> 31);
+                    s[kb][i] = __uint_as_float((__float_as_uint(s[kb][i]) & keep) | (0xff800000u & ~keep));
                 }
+            }
         }
         float mx = NEG_BIG;
 #pragma unroll
@@ -330,14 +359,13 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 ? 1 : 2) void window_tile_kerne
         for (int kb = 0; kb < KB; ++kb) {
             if constexpr (sizeof(E) == 4) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int key = 32 * kb + 8 * (i >> 2) + 4 * h + (i & 3);
+                for (int i = 0; i < 16; ++i)
 #pragma unroll
                     for (int dt = 0; dt < DT; ++dt) {
-                        const float v = *reinterpret_cast<const float*>(vs + key * I::ROWB + (((dt * 8 + (r >> 2)) ^ I::v_swizzle(key)) * 16) + (r & 3) * 4);
+                        const int key = 32 * kb + 8 * (i >> 2) + 4 * h + (i & 3);
+                        const float v = *reinterpret_cast<const float*>(vs + key * I::ROWB + ((dt * 8 + (r >> 2)) ^ I::v_swizzle(key)) * 16 + (r & 3) * 4);
                         o[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, s[kb][i], o[dt], 0, 0, 0);
                     }
-                }
             } else {
                 typedef short tr4 __attribute__((__vector_size__(4 * sizeof(short))));
                 const int rho = (lane & 15) >> 2, col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
@@ -352,7 +380,7 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 ? 1 : 2) void window_tile_kerne
 #pragma unroll
                         for (int u = 0; u < 2; ++u) {
                             const int row = 32 * kb + 16 * tt + 8 * u + 4 * h + rho;
-                            const unsigned char* p = vs + row * I::ROWB + (((dt * 4 + (col >> 3)) ^ I::v_swizzle(row)) * 16) + (col & 4) * 2;
+                            const unsigned char* p = vs + row * I::ROWB + ((dt * 4 + (col >> 3)) ^ I::v_swizzle(row)) * 16 + (col & 4) * 2;
                             av.t[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) tr4*)p);
                         }
                         o[dt] = Mma<E>::mfma(av.v, pb, o[dt]);
@@ -819,12 +847,13 @@ int window_launch(const WinArgs& a, void* work, int64_t work_bytes, hipStream_t 
         return window_few<T, D, 4>(a, p, work, stream);
     }
     const int q_tiles = (a.max_q + 127) / 128;
-    const int64_t units = (int64_t)a.n_seq * q_tiles * a.hq;
-    const int64_t grid = (units + 7) / 8 * 8;
+    const int64_t pairs = (int64_t)a.n_seq * a.hkv, units = pairs * q_tiles * (a.hq / a.hkv);
+    const bool by_pair = pairs % 8 == 0 || pairs >= 64;
+    const int64_t grid = by_pair ? (pairs + 7) / 8 * 8 * q_tiles * (a.hq / a.hkv) : (units + 7) / 8 * 8;
     RAG_REQUIRE(grid < (1ll << 31), RAG_ELIMIT, "rag_enc_attention_window: too many query tiles");
-    constexpr size_t lds = 4 * (size_t)Image<T, D>::BYTES;
+    constexpr size_t lds = 2 * (size_t)Image<T, D>::BUFFERS * Image<T, D>::BYTES;
     RAG_GRANT_LDS((window_tile_kernel<T, D>), lds);
-    window_tile_kernel<T, D><<<(unsigned)grid, 256, lds, stream>>>(a, q_tiles, (uint32_t)units, rag_fault_word());
+    window_tile_kernel<T, D><<<(unsigned)grid, 256, lds, stream>>>(a, q_tiles, (uint32_t)units, by_pair, rag_fault_word());
     RAG_HIP_TRY(hipGetLastError());
     return RAG_OK;
 }
