@@ -207,12 +207,16 @@ __global__ __launch_bounds__(256, (Image<E, D>::WAVES)) void window_tile_kernel(
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
     // All units of a (sequence, key/value head) pair go to workgroups with the same blockIdx % 8, which round-robin
     // placement puts on one XCD: its L2 then holds their keys and values.  Fewer pairs than fill the XCDs evenly: an eighth of
-    // the units, neighbours, goes to each instead.
+    // the units, neighbours, goes to each instead.  Short pairs' units are turned by one from pair to pair: workgroups go
+    // round an XCD's 32 compute units, and where a pair's units divide that number the tiles that only long sequences have would
+    // all meet on the same ones (40 sequences of 1 to 512 tokens, 12 heads of 32, float32: 75 us, turned 63).  The last pair is not
+    // turned, so that its longest tiles do not end up alone.
     const uint32_t xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
     uint32_t unit = xcd * ((units + 7) >> 3) + at;
     if (by_pair) {
         const uint32_t per_pair = (uint32_t)(a.hq / a.hkv) * (uint32_t)q_tiles, turn = at / per_pair;
-        unit = (turn * 8 + xcd) * per_pair + (at - turn * per_pair);
+        const uint32_t shift = per_pair <= 32 ? (gridDim.x >> 3) / per_pair - 1 - turn : 0;
+        unit = (turn * 8 + xcd) * per_pair + (at - turn * per_pair + shift) % per_pair;
     }
     if (unit >= units) return;
     const int group = a.hq / a.hkv;
@@ -494,9 +498,13 @@ __device__ __forceinline__ float quarters_sum(float v) {
 struct FewArgs {
     int chunks;                      // of 16 * QT rows
     int spans, span;                 // workgroups along the keys, tiles of each
-    float2* part_ml;                 // [query row * head][spans]: maximum, sum
-    float* part_o;                   // [query row * head][spans][D]
+    bool by_seq;                     // a partial result's row: sequence * max_q + query instead of the query's row of q
+    float2* part_ml;                 // [row][head][spans]: maximum, sum
+    float* part_o;                   // [row][head][spans][D]
 };
+__device__ __forceinline__ int64_t part_at(const WinArgs& a, const FewArgs& f, const Seq& sq, int seq, int j, int head) {
+    return ((f.by_seq ? (int64_t)seq * a.max_q + j : sq.q0 + j) * a.hq + head) * f.spans;
+}
 
 template <typename E, int D, int QT>
 __global__ __launch_bounds__(64 * (FewImage<E, D>::NW)) void window_few_kernel(WinArgs a, FewArgs f, uint32_t* fault) {
@@ -702,7 +710,7 @@ __global__ __launch_bounds__(64 * (FewImage<E, D>::NW)) void window_few_kernel(W
             sum += *reinterpret_cast<const f32x4*>(sums + w * WAVE_F + lr * D + d) * weight;
         }
         if (f.spans > 1) {
-            const int64_t at = ((sq.q0 + j) * a.hq + head) * (int64_t)f.spans + span;
+            const int64_t at = part_at(a, f, sq, seq, j, head) + span;
             if (d == 0) f.part_ml[at] = make_float2(top, total);
             *reinterpret_cast<f32x4*>(f.part_o + at * D + d) = sum;
         } else {
@@ -744,7 +752,7 @@ __global__ __launch_bounds__(256) void window_join_kernel(WinArgs a, FewArgs f, 
     const int last = min((chunk + 1) * rows_of_chunk, sq.nq * group) - 1;
     const Tiles tiles = tiles_of(a, sq, chunk * rows_of_chunk / group, last / group, FewImage<E, D>::KT);
     const int n = max(1, (tiles.n + f.span - 1) / f.span);
-    const int64_t at = ((sq.q0 + j) * a.hq + head) * (int64_t)f.spans;
+    const int64_t at = part_at(a, f, sq, seq, j, head);
     const float scale = fabsf(a.scale);
     float top = NEG_BIG;
     for (int i = lane; i < n; i += 64) top = fmaxf(top, f.part_ml[at + i].x);
@@ -787,20 +795,39 @@ struct Plan {
     int qt, chunks, spans, span;     // few: 16-row columns of a workgroup, its row chunks, spans along the keys
     int64_t parts;                   // query rows * heads * spans whose partial results the workspace holds
 };
+
+// The most keys that `queries` neighbouring queries can see, in tiles of kt
+int64_t most_tiles(int max_k, int queries, int left, int right, int sinks, int kt) {
+    int64_t keys = max_k;
+    if (left >= 0) keys = std::min<int64_t>(keys, (int64_t)sinks + left + queries + (right < 0 ? max_k : std::min(right, max_k)));
+    return std::max<int64_t>(1, (keys + kt - 1) / kt + (left >= 0 ? 2 : 0));
+}
+
 Plan plan_of(int64_t total_q, int n_seq, int max_q, int max_k, int hq, int hkv, int D, int left, int right, int sinks, int size) {
     Plan p{};
-    const int group = hq / hkv;
+    const int group = hq / hkv, wide = size == 4, di = D == 32 ? 0 : D == 64 ? 1 : 2;
     const int64_t rows = (int64_t)max_q * group;
-    p.few = rows <= 64;
-    if (!p.few) return p;
     p.qt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
     p.chunks = (int)((rows + 16 * p.qt - 1) / (16 * p.qt));
-    const int kt = size == 4 ? 16 : 32;
-    // the most keys that the queries of a sequence can see
-    int64_t keys = max_k;
-    if (left >= 0) keys = std::min<int64_t>(keys, (int64_t)sinks + left + max_q + (right < 0 ? max_k : std::min(right, max_k)));
-    const int64_t tiles = std::max<int64_t>(1, (keys + kt - 1) / kt + (left >= 0 ? 2 : 0));
+    const int kt = wide ? 16 : 32;
+    const int64_t tiles = most_tiles(max_k, max_q, left, right, sinks, kt);
     const int64_t base = (int64_t)n_seq * hkv * p.chunks;
+
+    // Which kernel: both times estimated in microseconds.  The tile kernel walks the keys of 128 queries one tile after the
+    // other; the few-query kernel spreads them over the chip but reads them once per 64 rows, with a second launch and
+    // narrower matrix operands.  The constants are fitted to both kernels' times over 115 sizes a type and head size (1 to 64
+    // sequences, 5 to 200 queries, 300 to 16384 keys); by the estimate the sum of the chosen times is 1 % over the best of
+    // both, at worst a case 1.4 times.  E.g. head size 128, one sequence of 200 queries, 16 heads on 8, 16384 keys: tiles 331
+    // us, few 105; 64 sequences of them on 4096 keys: 565 and 1289.
+    static const double few_tile[2][3] = {{1.2, 1.7, 3.4}, {1.5, 2.4, 4.5}};
+    static const double one_tile[2][3] = {{0.9, 0.9, 1.17}, {1.0, 1.2, 1.5}}, all_tiles[2][3] = {{0.7, 0.8, 1.07}, {1.0, 1.7, 3.0}};
+    const double wgs = (double)n_seq * hq * ((max_q + 127) / 128), waves = std::min(4, (max_q + 31) / 32 + 1);
+    const double few_us = (p.qt == 4 ? 20 : 9) + (double)base * tiles / 1024 * few_tile[wide][di];
+    const double tile_us = 9 + (double)most_tiles(max_k, std::min(max_q, 128), left, right, sinks, wide ? 32 : 64) *
+                                   std::max(one_tile[wide][di], all_tiles[wide][di] * wgs * waves / 1024);
+    p.few = few_us < tile_us && base < (1 << 24);
+    if (!p.few) return p;
+
     // A workgroup's start, the filling of its buffers and its end cost as much as some 8 tiles a wave, so the workgroups that are on
     // the chip at once (256 compute units by what their LDS leaves room for) run one round: one token over 32768 keys of 8 heads
     // 36.6 us, in two rounds 44, in three 51.  Spans that would be long all the same (over 256 tiles) are cut in three, against
@@ -811,7 +838,7 @@ Plan plan_of(int64_t total_q, int n_seq, int max_q, int max_k, int hq, int hkv, 
     if (tiles / cuts > 256) cuts = std::max<int64_t>(1, 3 * on_chip / base);
     p.span = (int)(tiles <= 20 ? tiles : std::max<int64_t>(8, (tiles + cuts - 1) / cuts));
     p.spans = (int)((tiles + p.span - 1) / p.span);
-    p.parts = p.spans > 1 ? total_q * hq * p.spans : 0;
+    p.parts = p.spans > 1 ? std::min(total_q, (int64_t)n_seq * max_q) * hq * p.spans : 0;
     return p;
 }
 
@@ -819,6 +846,7 @@ template <typename T, int D, int QT>
 int window_few(const WinArgs& a, const Plan& p, void* work, hipStream_t stream) {
     FewArgs f;
     f.chunks = p.chunks; f.spans = p.spans; f.span = p.span;
+    f.by_seq = (int64_t)a.n_seq * a.max_q < a.total_q;       // rows of no sequence take no room
     f.part_o = reinterpret_cast<float*>(work);
     f.part_ml = reinterpret_cast<float2*>(f.part_o + p.parts * D);
     const int64_t grid = (int64_t)a.n_seq * p.spans * p.chunks * a.hkv;
