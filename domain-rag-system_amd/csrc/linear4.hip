@@ -86,8 +86,8 @@ template <> struct XFrag<float> {
     }
 };
 
-// (1024 threads leave 128 registers a lane: enough for one row tile of 16-bit x)
-template <typename T, int MT> constexpr int max_waves() { return MT == 1 && sizeof(T) == 2 ? 16 : 8; }
+// (1024 threads leave 128 registers a lane: enough for one or two row tiles and 16-bit x)
+template <typename T, int RT> constexpr int max_waves() { return RT <= 2 && sizeof(T) == 2 ? 16 : 8; }
 
 // A group's scale and offset as one value
 template <typename T> struct ScalePair {
@@ -125,7 +125,7 @@ template <> struct ScalePair<float> {
 // The loads of the wave's next block are issued before the products of this one.  Loads return in order: x, which comes from the L2, is
 // asked for before the codes of the next block, which come from memory, or with its own block (MT == 1).
 template <typename T, int MT, int RT, int GROUP>
-__global__ __launch_bounds__((64 * max_waves<T, MT>())) void linear4_kernel(Lin4Args a) {
+__global__ __launch_bounds__((64 * max_waves<T, RT>())) void linear4_kernel(Lin4Args a) {
     typedef XFrag<T> XF;
     typedef typename XF::E E;
     typedef Code16<E> C16;
@@ -330,7 +330,7 @@ int linear4_by_group(Lin4Args a, hipStream_t stream) {
     const int64_t my = ceil_div64(a.m, 16 * MT);
     RAG_REQUIRE(my <= 65535, RAG_ELIMIT, "rag_enc_linear4: too many rows of x");
     int waves = 4;
-    while (waves < max_waves<T, MT>() && waves < blocks && (int64_t)tiles * my * waves < 4096) waves *= 2;
+    while (waves < max_waves<T, RT>() && waves < blocks && (int64_t)tiles * my * waves < 2048) waves *= 2;
     const dim3 grid((unsigned)tiles, (unsigned)my);
     // at most 32 KB of scales at a time
     const int ng = 128 / a.group, row_bytes = 16 * RT * (int)sizeof(typename ScalePair<T>::type);
@@ -343,17 +343,17 @@ int linear4_by_group(Lin4Args a, hipStream_t stream) {
     return RAG_OK;
 }
 
-template <typename T, int MT>
-int linear4_by_rows(const Lin4Args& a, hipStream_t stream) {
-    if (a.n >= 8192) return linear4_by_group<T, MT, 2>(a, stream);
-    return linear4_by_group<T, MT, 1>(a, stream);
-}
-
+// The smallest tile with which the workgroups are on the chip at once, one per compute unit: x is read by each of them, so
+// fewer and larger ones read less, but a second round costs as much as the first (k 4096, group 128: n 4096, m 16: 16 x 16 tiles
+// 10 us, 32 x 16 12; m 64: 16 x 16 23, 32 x 16 17, 64 x 16 13.2, and 16 x 64, 256 workgroups too, 19.9).  Beyond that the
+// largest, up to 8 rows of x 32 x 16, which keep more waves on the chip for the weights (n 16383, k 8192, m 1: 21 us, 64 x 16 26).
 template <typename T>
 int linear4_launch(const Lin4Args& a, hipStream_t stream) {
-    if (a.m <= 16) return linear4_by_rows<T, 1>(a, stream);
-    if (a.m <= 32) return linear4_by_rows<T, 2>(a, stream);
-    return linear4_by_rows<T, 4>(a, stream);
+    const int64_t tiles = (a.n + 15) / 16, my = (a.m + 15) / 16;
+    if (tiles * my <= 256) return linear4_by_group<T, 1, 1>(a, stream);
+    if (a.m <= 8 || (tiles + 1) / 2 * my <= 256) return linear4_by_group<T, 1, 2>(a, stream);
+    if (a.m <= 16 || (tiles + 3) / 4 * my <= 256) return linear4_by_group<T, 1, 4>(a, stream);
+    return linear4_by_group<T, 2, 4>(a, stream);
 }
 
 }  // namespace
