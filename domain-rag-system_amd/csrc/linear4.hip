@@ -132,6 +132,8 @@ __global__ __launch_bounds__((64 * max_waves<T, RT>())) void linear4_kernel(Lin4
     typedef typename C16::x8 x8;
     constexpr int NG = 128 / GROUP;                          // groups of a block
     constexpr int SPG = GROUP / 32;                          // steps of a group
+    constexpr int RUN = sizeof(T) == 4 ? 1 : SPG;            // steps summed before the scale: c, five times the size of what is left of it, is
+                                                             // kept short where its last bits count (group 128: error 8e-7, a step 5e-7)
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 63, waves = (int)(blockDim.x >> 6);
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -201,8 +203,8 @@ __global__ __launch_bounds__((64 * max_waves<T, RT>())) void linear4_kernel(Lin4
             w[u][2] = p[0]; w[u][3] = p[1];
         }
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            if (g * SPG >= steps) break;                     // (k is a whole number of groups)
+        for (int step0 = 0; step0 < 4; step0 += RUN) {
+            if (step0 >= steps) break;                       // (k is a whole number of groups)
             f32x4 c[RT][MT], X[MT];
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
@@ -211,8 +213,7 @@ __global__ __launch_bounds__((64 * max_waves<T, RT>())) void linear4_kernel(Lin4
                 for (int u = 0; u < RT; ++u) c[u][t] = f32x4{0.f, 0.f, 0.f, 0.f};
             }
 #pragma unroll
-            for (int i = 0; i < SPG; ++i) {
-                const int step = g * SPG + i;
+            for (int step = step0; step < step0 + RUN; ++step) {
                 x8 code[RT];
 #pragma unroll
                 for (int u = 0; u < RT; ++u) code[u] = __builtin_bit_cast(x8, C16::unpack(w[u][step], mask, base));
@@ -232,7 +233,7 @@ __global__ __launch_bounds__((64 * max_waves<T, RT>())) void linear4_kernel(Lin4
 #pragma unroll
             for (int u = 0; u < RT; ++u) {
                 float s, off;
-                ScalePair<T>::split(pairs[(16 * u + r) * pair_stride + g0 + g], s, off);
+                ScalePair<T>::split(pairs[(16 * u + r) * pair_stride + g0 + step0 / SPG], s, off);
                 off = fmaf(s_mul, s, off * o_mul);
 #pragma unroll
                 for (int t = 0; t < MT; ++t)
