@@ -204,6 +204,36 @@ def test_extreme_scores():
 
 
 @pytest.mark.parametrize('kind', list(TYPES))
+@pytest.mark.parametrize('nq,nk', [(1, 3000), (200, 200)])
+def test_other_scales(kind, nq, nk):
+    """A scale of zero (the mean of what is seen), tiny, large and negative ones, in both kernels."""
+    import rag_hip
+    g, dt = _gen(12), TYPES[kind]
+    q = torch.randn((nq, 4, 64), generator=g, device=_dev()).to(dt)
+    k, v = (torch.randn((nk, 2, 64), generator=g, device=_dev()).to(dt) for _ in range(2))
+    for scale in (0.0, 1e-30, 1e-3, 2.0, -0.125):
+        got = rag_hip.enc_attention_window_dev(q, k, v, _cu([nq]), nq, k_start=torch.zeros(1, dtype=torch.int64, device=_dev()),
+                                               k_len=torch.tensor([nk], dtype=torch.int32, device=_dev()), max_k_len=nk, window_left=150, window_right=0,
+                                               n_sinks=3, scale=scale)
+        _check(got, q, k, v, [nq], [(0, nk)], 150, 0, 3, scale)
+
+
+@pytest.mark.parametrize('hq,hkv', [(8, 8), (8, 1), (40, 1)])
+def test_sequences_among_rows_of_none(hq, hkv):
+    """Two short sequences somewhere in a long array of queries, over many keys (partial results are kept by sequence)."""
+    import rag_hip
+    g, rows = _gen(13), 5000
+    q = torch.randn((rows, hq, 64), generator=g, device=_dev()).to(torch.bfloat16)
+    k, v = (torch.randn((6000, hkv, 64), generator=g, device=_dev()).to(torch.bfloat16) for _ in range(2))
+    out = torch.full((rows, hq * 64), 7.0, dtype=torch.bfloat16, device=_dev())
+    cu = torch.tensor([4000, 4003, 4005], dtype=torch.int32, device=_dev())
+    rag_hip.enc_attention_window_dev(q, k, v, cu, 3, k_start=torch.tensor([0, 500], device=_dev()), k_len=torch.tensor([6000, 5500], dtype=torch.int32, device=_dev()),
+                                     max_k_len=6000, window_right=0, out=out)
+    _check(out[4000:4005], q[4000:4005], k, v, [3, 2], [(0, 6000), (500, 5500)], -1, 0, 0, 0.125)
+    assert bool((out[:4000] == 7).all()) and bool((out[4005:] == 7).all())
+
+
+@pytest.mark.parametrize('kind', list(TYPES))
 @pytest.mark.parametrize('max_q', [4, 80])
 def test_bad_sequences_are_flagged_and_rows_of_none_stay(kind, max_q):
     import rag_hip

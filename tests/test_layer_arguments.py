@@ -40,7 +40,7 @@ def _window(**kw):
 
 @pytest.mark.parametrize('kw,code', [
     (dict(dt=3), -1), (dict(d=48), -5), (dict(n=-1), -1), (dict(mq=-1), -1), (dict(tq=-1), -1), (dict(tk=-1), -1), (dict(tq=1 << 31), -5), (dict(mk=1 << 30), -5),
-    (dict(hq=3, hkv=2), -1), (dict(hkv=0), -1), (dict(left=-2), -1), (dict(right=-2), -1), (dict(sinks=-1), -1), (dict(scale=float('inf')), -1),
+    (dict(hq=3, hkv=2), -1), (dict(hkv=0), -1), (dict(left=-2), -1), (dict(right=-2), -1), (dict(sinks=-1), -1), (dict(scale=float('inf')), -1), (dict(scale=3e38), -1),
     (dict(q=None), -1), (dict(k=None), -1), (dict(out=None), -1), (dict(cu=None), -1), (dict(qs=24), -1), (dict(qs=33), -1), (dict(os=16), -1), (dict(krs=4), -1), (dict(bytes=-1), -1)])
 def test_window_arguments(kw, code):
     rc, text = _window(**kw)
@@ -50,6 +50,25 @@ def test_window_arguments(kw, code):
 def test_window_starts_and_lengths_come_together():
     keep, p = _buf(64)
     assert _window(ks=p)[0] == -1 and _window(kl=p)[0] == -1
+
+
+def test_workspace_goes_by_the_sizes_and_never_overflows():
+    import rag_hip
+    f = rag_hip.load_library().rag_enc_attention_window_workspace
+    one = f(1, 1, 1, 32768, 32, 8, 128, -1, 0, 0, 1)
+    assert one > 0 and one % (32 * 130 * 4) == 0               # spans of one token's 32 heads: 128 sums, a maximum and a total
+    assert f(1 << 30, 1, 1, 32768, 32, 8, 128, -1, 0, 0, 1) == one       # rows of no sequence take no room
+    assert f(16384, 1, 16384, 16384, 16, 8, 128, 4096, 0, 4, 1) == 0 and f(0, 0, 0, 0, 1, 1, 64, -1, -1, 0, 0) == 0
+    big = (1 << 31) - 1
+    for dtype in (0, 1, 2):
+        for args in ((big, big, 1, (1 << 30) - 1, 4096, 1, 128), (big, 1, (1 << 30) - 1, (1 << 30) - 1, 4096, 1, 32), (big, 1, 1, (1 << 30) - 1, 4096, 4096, 128)):
+            for window in ((-1, -1, 0), (big, big, big), (0, 0, big)):
+                assert 0 <= f(*args, *window, dtype) < 1 << 50
+
+
+def test_a_workspace_too_small_is_refused():
+    # refused before any launch: 32768 keys in spans need room for their partial results
+    assert _window(hq=32, hkv=8, d=128, qs=4096, os=4096, tq=1, mk=32768, tk=32768, ks=_buf(64)[1], kl=_buf(64)[1])[0] == -1
 
 
 def test_nothing_to_do_is_no_error():
