@@ -2,9 +2,13 @@
 // w[n][k] = scale[n][k / G] * code[n][k] + offset[n][k / G] (no offsets: scale * (code - 8)).  The dense layers of an
 // encoder for one query's tokens (MedicalEmbedder.encode of one text, reference src/indexing/embedder.py:65-71), where
 // reading the weights is what the layer costs.  gfx950 only.
+// Measured, bf16, group 32, n 16383, k 8192 (75 MB): one token 20.7 us (3.6 TB/s; a large copy moves 4.7), 13 tokens 24 (147
+// TFLOP/s of products: the codes are unpacked by the vector units beside them, and the waves meet once per workgroup), 64
+// tokens 54; n 4096, k 4096, group 128 (8.9 MB): 5.3, 6.2 and 10.
 #include "common.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -21,6 +25,7 @@ struct Lin4Args {
     void* y;
     int64_t x_stride, y_stride, m;
     int32_t n, k, group;
+    int32_t image;                   // where the images of x begin in LDS
     int32_t chunk;                   // 128-column blocks whose scales are in LDS at a time
 };
 
@@ -51,6 +56,8 @@ template <typename T> struct XFrag {
     static constexpr int PARTS = 1;
     uint4 v;
     __device__ void load(const T* p) { v = *reinterpret_cast<const uint4*>(p); }
+    // columns 8 piece .. of a row of an image in LDS whose 16-byte pieces lie at p ^ s
+    __device__ void load(const unsigned char* row, int piece, int s) { v = *reinterpret_cast<const uint4*>(row + (piece ^ s) * 16); }
     __device__ void parts(uint4* out) const {
         out[0].x = __builtin_amdgcn_perm(v.z, v.x, 0x05040100u);
         out[0].y = __builtin_amdgcn_perm(v.z, v.x, 0x07060302u);
@@ -65,6 +72,10 @@ template <> struct XFrag<float> {
     __device__ void load(const float* p) {
         a = *reinterpret_cast<const float4*>(p);
         b = *reinterpret_cast<const float4*>(p + 4);
+    }
+    __device__ void load(const unsigned char* row, int piece, int s) {
+        a = *reinterpret_cast<const float4*>(row + ((2 * piece) ^ s) * 16);
+        b = *reinterpret_cast<const float4*>(row + ((2 * piece + 1) ^ s) * 16);
     }
     __device__ static void cut(float lo, float hi, uint32_t* out) {
 #pragma unroll
@@ -124,7 +135,9 @@ template <> struct ScalePair<float> {
 //
 // The loads of the wave's next block are issued before the products of this one.  Loads return in order: x, which comes from the L2, is
 // asked for before the codes of the next block, which come from memory, or with its own block (MT == 1).
-template <typename T, int MT, int RT, int GROUP>
+// x is loaded as the operands lie (16 rows, 64 bytes of each a load), or with ROWS in whole pieces of few rows, which go
+// through an image in LDS: rows of x lie a power of two apart as a rule, so that 16 of them meet on one channel of the L2.
+template <typename T, int MT, int RT, int GROUP, bool ROWS>
 __global__ __launch_bounds__((64 * max_waves<T, RT>())) void linear4_kernel(Lin4Args a) {
     typedef XFrag<T> XF;
     typedef typename XF::E E;
@@ -153,12 +166,23 @@ __global__ __launch_bounds__((64 * max_waves<T, RT>())) void linear4_kernel(Lin4
     for (int t = 0; t < RT; ++t) {
         code_at[t] = (uint32_t)min(16 * t + r, rows_here - 1) * (uint32_t)(a.k / 2) + 16 * q;    // (rows beyond the last repeat it and are not stored)
     }
+    constexpr int X_ROWB = 128 * (int)sizeof(T), X_PIECES = X_ROWB / 16, X_ROWS = 1024 / X_ROWB, X_LOADS = MT * X_ROWB / 64;
+    const uint8_t* xbase = reinterpret_cast<const uint8_t*>(a.x) + m0 * a.x_stride * (int64_t)sizeof(T);
+    const int m_here = (int)min((int64_t)(16 * MT), a.m - m0);
+    uint32_t x_at[X_LOADS];                                  // ROWS: the lane's rows of x, in bytes (they fit by the limit on the stride)
+#pragma unroll
+    for (int i = 0; i < X_LOADS; ++i)
+        x_at[i] = (uint32_t)min(i * X_ROWS + lane / X_PIECES, m_here - 1) * (uint32_t)(a.x_stride * (int64_t)sizeof(T));
+    unsigned char* image = smem + a.image + wave * (16 * MT * X_ROWB);
     const T* x[MT];
 #pragma unroll
     for (int t = 0; t < MT; ++t) x[t] = reinterpret_cast<const T*>(a.x) + min(m0 + 16 * t + r, a.m - 1) * a.x_stride + 8 * q;
 
     struct Block { uint4 w[RT]; };
-    struct XBlock { XF f[4][MT]; };
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    struct XRows { u32x4 raw[X_LOADS]; };
+    struct XFrags { XF f[4][MT]; };
+    typedef typename std::conditional<ROWS, XRows, XFrags>::type XBlock;
     auto load = [&](int blk, Block& b) {
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
@@ -166,11 +190,18 @@ __global__ __launch_bounds__((64 * max_waves<T, RT>())) void linear4_kernel(Lin4
         }
     };
     auto load_x = [&](int blk, XBlock& b) {
+        if constexpr (ROWS) {
+            const int last = min(128, a.k - 128 * blk) * (int)sizeof(T) / 16 - 1;         // (in a row's last block: pieces beyond it repeat it)
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            const T* p = x[t] + 128 * blk;
+            for (int i = 0; i < X_LOADS; ++i)
+                b.raw[i] = *reinterpret_cast<const u32x4*>(xbase + (int64_t)blk * X_ROWB + (x_at[i] + 16 * min(lane % X_PIECES, last)));
+        } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) b.f[i][t].load(p + 32 * i);
+            for (int t = 0; t < MT; ++t) {
+                const T* p = x[t] + 128 * blk;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) b.f[i][t].load(p + 32 * i);
+            }
         }
     };
     f32x4 y[RT][MT];
@@ -190,6 +221,14 @@ __global__ __launch_bounds__((64 * max_waves<T, RT>())) void linear4_kernel(Lin4
     const int pair_stride = (a.chunk * NG) | 1;
     // g0: the block's first group in the chunk
     auto process = [&](const Block& cur, const XBlock& xcur, int g0, int steps) {
+        if constexpr (ROWS) {                                // (LDS accesses of a wave stay in order)
+#pragma unroll
+            for (int i = 0; i < X_LOADS; ++i) {
+                const int row = i * X_ROWS + lane / X_PIECES;
+                *reinterpret_cast<u32x4*>(image + row * X_ROWB + ((lane % X_PIECES) ^ (row & 15)) * 16) = xcur.raw[i];
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
         uint32_t w[RT][4];
 #pragma unroll
         for (int u = 0; u < RT; ++u) {
@@ -220,7 +259,13 @@ __global__ __launch_bounds__((64 * max_waves<T, RT>())) void linear4_kernel(Lin4
 #pragma unroll
                 for (int t = 0; t < MT; ++t) {
                     uint4 part[XF::PARTS];
-                    xcur.f[step][t].parts(part);
+                    if constexpr (ROWS) {
+                        XF xf;
+                        xf.load(image + (16 * t + r) * X_ROWB, 4 * step + q, r);
+                        xf.parts(part);
+                    } else {
+                        xcur.f[step][t].parts(part);
+                    }
 #pragma unroll
                     for (int p = 0; p < XF::PARTS; ++p) {
                         const x8 xa = __builtin_bit_cast(x8, part[p]);
@@ -296,10 +341,14 @@ __global__ __launch_bounds__((64 * max_waves<T, RT>())) void linear4_kernel(Lin4
             const int col = min(128 * full + 32 * q, a.k - 32);
 #pragma unroll
             for (int t = 0; t < RT; ++t) b0.w[t] = *reinterpret_cast<const uint4*>(codes + (code_at[t] - 16 * q + (uint32_t)(col >> 1)));
+            if constexpr (ROWS) {
+                load_x(full, x0);
+            } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int t = 0; t < MT; ++t) x0.f[i][t].load(x[t] + min(128 * full + 32 * i, a.k - 32));
+                    for (int t = 0; t < MT; ++t) x0.f[i][t].load(x[t] + min(128 * full + 32 * i, a.k - 32));
+            }
             process(b0, x0, (full - c0) * NG, (a.k % 128) / 32);
         }
         __syncthreads();                                     // the scales are read: the next chunk's, or the sums, go there
@@ -325,7 +374,7 @@ __global__ __launch_bounds__((64 * max_waves<T, RT>())) void linear4_kernel(Lin4
     }
 }
 
-template <typename T, int MT, int RT>
+template <typename T, int MT, int RT, bool ROWS>
 int linear4_by_group(Lin4Args a, hipStream_t stream) {
     const int tiles = (a.n + 16 * RT - 1) / (16 * RT), blocks = (a.k + 127) / 128;
     const int64_t my = ceil_div64(a.m, 16 * MT);
@@ -333,28 +382,47 @@ int linear4_by_group(Lin4Args a, hipStream_t stream) {
     int waves = 4;
     while (waves < max_waves<T, RT>() && waves < blocks && (int64_t)tiles * my * waves < 2048) waves *= 2;
     const dim3 grid((unsigned)tiles, (unsigned)my);
-    // at most 32 KB of scales at a time
+    // at most 32 KB of scales at a time (24 where the images of x take 128)
     const int ng = 128 / a.group, row_bytes = 16 * RT * (int)sizeof(typename ScalePair<T>::type);
-    a.chunk = std::min(blocks, 32768 / (row_bytes * ng));
-    const size_t lds = std::max((size_t)row_bytes * ((a.chunk * ng) | 1), (size_t)waves * MT * RT * 1024);
-    if (a.group == 32) linear4_kernel<T, MT, RT, 32><<<grid, 64 * waves, lds, stream>>>(a);
-    else if (a.group == 64) linear4_kernel<T, MT, RT, 64><<<grid, 64 * waves, lds, stream>>>(a);
-    else linear4_kernel<T, MT, RT, 128><<<grid, 64 * waves, lds, stream>>>(a);
+    const int images = ROWS ? waves * 16 * MT * 128 * (int)sizeof(T) : 0;
+    a.chunk = std::min(blocks, (images > 65536 ? 24576 : 32768) / (row_bytes * ng));
+    a.image = (row_bytes * ((a.chunk * ng) | 1) + 1023) / 1024 * 1024;
+    const size_t lds = std::max((size_t)a.image + images, (size_t)waves * MT * RT * 1024);
+#define RAG_LINEAR4_LAUNCH(G)                                                            \
+    do {                                                                                 \
+        RAG_GRANT_LDS((linear4_kernel<T, MT, RT, G, ROWS>), lds);                         \
+        linear4_kernel<T, MT, RT, G, ROWS><<<grid, 64 * waves, lds, stream>>>(a);         \
+    } while (0)
+    if (a.group == 32) RAG_LINEAR4_LAUNCH(32);
+    else if (a.group == 64) RAG_LINEAR4_LAUNCH(64);
+    else RAG_LINEAR4_LAUNCH(128);
+#undef RAG_LINEAR4_LAUNCH
     RAG_HIP_TRY(hipGetLastError());
     return RAG_OK;
 }
 
+// x by whole rows from 5 rows on (n 4096, k 4096: m 4 6.1 us as operands, 6.0 by rows, m 13 7.9 and 6.2); not where fp32
+// rows and 64 rows of weights are more than the registers hold (n 16383, k 8192, m 24: 57 us, by rows 71).
+template <typename T, int MT, int RT>
+int linear4_tile(const Lin4Args& a, hipStream_t stream) {
+    if constexpr (sizeof(T) == 2 || RT < 4)
+        if (a.m > 4) return linear4_by_group<T, MT, RT, true>(a, stream);
+    if constexpr (sizeof(T) == 4 || RT < 4) return linear4_by_group<T, MT, RT, false>(a, stream);
+    return RAG_EINVAL;                                       // (64 rows of weights are for more than 16 of x)
+}
+
 // The smallest tile with which the workgroups are on the chip at once, one per compute unit: x is read by each of them, so
-// fewer and larger ones read less, but a second round costs as much as the first (k 4096, group 128: n 4096, m 16: 16 x 16 tiles
-// 10 us, 32 x 16 12; m 64: 16 x 16 23, 32 x 16 17, 64 x 16 13.2, and 16 x 64, 256 workgroups too, 19.9).  Beyond that the
-// largest, up to 8 rows of x 32 x 16, which keep more waves on the chip for the weights (n 16383, k 8192, m 1: 21 us, 64 x 16 26).
+// fewer and larger ones read less, but a second round costs as much as the first (k 4096, group 128, x as operands: n 4096, m 16: 16 x 16
+// tiles 10 us, 32 x 16 12; m 64: 16 x 16 23, 32 x 16 17, 64 x 16 13.2, and 16 x 64, 256 workgroups too, 19.9).  Beyond that the
+// largest, up to 16 rows of x 32 x 16, which keep more waves on the chip for the weights (n 16383, k 8192: m 1 21 us, 64 x 16 26; m
+// 13 23.8 and 26.9).
 template <typename T>
 int linear4_launch(const Lin4Args& a, hipStream_t stream) {
     const int64_t tiles = (a.n + 15) / 16, my = (a.m + 15) / 16;
-    if (tiles * my <= 256) return linear4_by_group<T, 1, 1>(a, stream);
-    if (a.m <= 8 || (tiles + 1) / 2 * my <= 256) return linear4_by_group<T, 1, 2>(a, stream);
-    if (a.m <= 16 || (tiles + 3) / 4 * my <= 256) return linear4_by_group<T, 1, 4>(a, stream);
-    return linear4_by_group<T, 2, 4>(a, stream);
+    if (tiles * my <= 256) return linear4_tile<T, 1, 1>(a, stream);
+    if (a.m <= 16 || (tiles + 1) / 2 * my <= 256) return linear4_tile<T, 1, 2>(a, stream);
+    if ((tiles + 3) / 4 * my <= 256) return linear4_tile<T, 1, 4>(a, stream);
+    return linear4_tile<T, 2, 4>(a, stream);
 }
 
 }  // namespace
@@ -367,7 +435,7 @@ extern "C" int rag_enc_linear4_dev(const void* d_x, int64_t x_stride, const uint
     RAG_REQUIRE(m >= 0 && n >= 1 && k >= 1, RAG_EINVAL, "%s: bad sizes", me);
     RAG_REQUIRE(group == 32 || group == 64 || group == 128, RAG_ELIMIT, "%s: the group must be 32, 64 or 128 (got %d)", me, group);
     RAG_REQUIRE(k % group == 0, RAG_ELIMIT, "%s: k = %d is not a multiple of the group %d", me, k, group);
-    RAG_REQUIRE(m < (1ll << 31) && n < (1 << 30) && k < (1 << 26), RAG_ELIMIT, "%s: sizes beyond the limit", me);
+    RAG_REQUIRE(m < (1ll << 31) && n < (1 << 28) && k < (1 << 26), RAG_ELIMIT, "%s: sizes beyond the limit", me);
     if (m == 0) return RAG_OK;
     RAG_REQUIRE(d_x && d_codes && d_scales && d_y, RAG_EINVAL, "%s: null pointer", me);
     const int size = dtype == RAG_DTYPE_F32 ? 4 : 2;
@@ -377,7 +445,8 @@ extern "C" int rag_enc_linear4_dev(const void* d_x, int64_t x_stride, const uint
                 reinterpret_cast<uintptr_t>(d_bias) % size == 0 && reinterpret_cast<uintptr_t>(d_y) % size == 0, RAG_EINVAL,
                 "%s: misaligned pointer", me);
     RAG_REQUIRE((m == 1 || x_stride >= k) && (m == 1 || y_stride >= n), RAG_EINVAL, "%s: a row's stride is smaller than the row", me);
-    Lin4Args a{d_x, d_codes, d_scales, d_offsets, d_bias, d_y, x_stride, y_stride, m, n, k, group, 0};
+    RAG_REQUIRE(m == 1 || x_stride <= (1 << 25) / size, RAG_ELIMIT, "%s: rows of x lie at most 32 MB apart", me);
+    Lin4Args a{d_x, d_codes, d_scales, d_offsets, d_bias, d_y, x_stride, y_stride, m, n, k, group, 0, 0};
     hipStream_t stream = (hipStream_t)stream_;
     if (dtype == RAG_DTYPE_F32) return linear4_launch<float>(a, stream);
     if (dtype == RAG_DTYPE_BF16) return linear4_launch<bf16>(a, stream);

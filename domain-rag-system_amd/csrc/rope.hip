@@ -12,6 +12,8 @@
 // a token: a lane's four are computed once and used for all heads the wave takes.  They are reduced to a fraction of
 // a turn in 64 bits (a 32-bit product is off by 2^-24 of the angle itself, 0.002 radians at position 32768) and only
 // the sine and cosine of the remainder are taken in 32 bits, so there is no table to read or to size.
+// Measured: 16384 tokens of 32 query and 8 key heads of 128, bf16, 70.6 us, 4.75 TB/s (a large copy moves 4.7); 65536 tokens
+// of 16 and 8 heads of 128, half of each rotated, f16, 161 us, 5.0 TB/s; one token 4.2 us, the launch.
 #include "common.h"
 
 namespace {

@@ -939,7 +939,7 @@ extern "C" int rag_enc_attention_window_dev(const void* d_q, int64_t q_stride, c
                 v_head_stride * size % 16 == 0 && out_stride * size % 16 == 0, RAG_EINVAL, "%s: strides must be multiples of 16 bytes", me);
     RAG_REQUIRE(q_stride >= (int64_t)n_q_heads * head_dim && out_stride >= (int64_t)n_q_heads * head_dim, RAG_EINVAL,
                 "%s: a row's stride is smaller than the row", me);
-    RAG_REQUIRE(llabs(k_row_stride) * size <= (1 << 25) && llabs(v_row_stride) * size <= (1 << 25) && k_row_stride >= 0 && v_row_stride >= 0, RAG_ELIMIT,
+    RAG_REQUIRE(k_row_stride >= 0 && v_row_stride >= 0 && k_row_stride <= (1 << 25) / size && v_row_stride <= (1 << 25) / size, RAG_ELIMIT,
                 "%s: rows of keys and values lie at most 32 MB apart", me);
     RAG_REQUIRE(workspace_bytes >= 0, RAG_EINVAL, "%s: bad workspace", me);
     WinArgs a;

@@ -576,9 +576,10 @@ int rag_enc_qk_norm_rope_dev(const void* d_qkv, int64_t qkv_stride, const int32_
  * out[row] = sum over the seen keys of softmax(scale q.k) v, head h with key/value head h / (n_q_heads / n_kv_heads);
  * a query that sees no key gets 0.  Keys and values a query does not see do not enter its result, whatever they hold.
  * Rows of q that belong to no sequence are not read, the same rows of out not written.  A sequence longer than
- * max_q_len / max_k_len or reaching beyond its arrays is skipped and flagged (RAG_FAULT_SEGMENT, RAG_FAULT_KV_ROW).
+ * max_q_len / max_k_len or reaching beyond its arrays is skipped and flagged (RAG_FAULT_SEGMENT, RAG_FAULT_KV_ROW);
+ * without k_start, max_q_len stands for max_k_len, here and in the workspace's size.
  * dtype bf16, fp16 (matrix cores, fp32 softmax and sums) or fp32; head_dim 32, 64 or 128; pointers and strides multiples
- * of 16 bytes; out must not overlap q, k or v.  workspace: rag_enc_attention_window_workspace() bytes for the same sizes (0:
+ * of 16 bytes, rows of k and v at most 32 MB apart; out must not overlap q, k or v.  workspace: rag_enc_attention_window_workspace() bytes for the same sizes (0:
  * may be NULL), 16-byte aligned, used by this call alone until it has run on its stream.                    */
 int64_t rag_enc_attention_window_workspace(int64_t total_q, int32_t n_seq, int32_t max_q_len, int32_t max_k_len,
                                            int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
@@ -593,8 +594,9 @@ int rag_enc_attention_window_dev(const void* d_q, int64_t q_stride, const void* 
 /* y[m][n] = sum_k x[m][k] w[n][k] + bias[n] with weights of 4 bits: w[n][k] = scales[n][k / group] * code + offsets[n][k / group],
  * without offsets (NULL) scales[n][k / group] * (code - 8).  codes [n][k / 2]: column 2i in the low half of byte i of
  * the row, column 2i + 1 in its high half; scales, offsets [n][k / group], bias [n] (or NULL) of x's type (bf16, fp16 or
- * fp32).  Made for the few rows of one query (weights are read once per 64 rows of x); any m works.  fp32 sums.
- * group 32, 64 or 128, k a multiple of it; x, its rows and the codes aligned to 16 bytes; y must not overlap x.   */
+ * fp32).  Made for the few rows of one query (the weights are read once per 16 or 32 rows of x).  fp32 sums.
+ * group 32, 64 or 128, k < 2^26 a multiple of it, n < 2^28, m up to 2 million; x, its rows and the codes aligned to 16 bytes, rows of
+ * x at most 32 MB apart; y must not overlap x.  A row of x that holds an infinity or a NaN gives infinities or NaN.   */
 int rag_enc_linear4_dev(const void* d_x, int64_t x_stride, const uint8_t* d_codes, const void* d_scales,
                         const void* d_offsets, const void* d_bias, int64_t m, int32_t n, int32_t k, int32_t group,
                         int32_t dtype, void* d_y, int64_t y_stride, void* stream);

@@ -91,6 +91,19 @@ def test_linear4_arguments(kw, code):
     assert rc == code and 'rag_enc_linear4' in text
 
 
+@pytest.mark.parametrize('kw', [
+    dict(n=1 << 28), dict(k=1 << 26), dict(m=2, xs=(1 << 24) + 8), dict(m=2, xs=1 << 62), dict(m=2, dt=0, xs=(1 << 23) + 4)])
+def test_linear4_limits(kw):
+    rc, text = _linear(**kw)
+    assert rc == -5 and 'rag_enc_linear4' in text
+
+
+@pytest.mark.parametrize('kw', [dict(krs=(1 << 24) + 8), dict(vrs=(1 << 24) + 8), dict(krs=-32), dict(vrs=1 << 61), dict(dt=0, krs=(1 << 23) + 4)])
+def test_window_rows_far_apart_are_refused(kw):
+    rc, text = _window(**kw)
+    assert rc == -5 and 'rag_enc_attention_window' in text
+
+
 @pytest.mark.parametrize('symmetric', [False, True])
 def test_quantize4_on_the_cpu(symmetric):
     import rag_hip
