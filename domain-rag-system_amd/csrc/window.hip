@@ -9,9 +9,10 @@
 #include "common.h"
 
 #include <algorithm>
+#include <atomic>
+#include <chrono>
 
 #include <math.h>
-#include <stdlib.h>
 
 namespace {
 
@@ -445,10 +446,10 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 // The rows of one key/value head's queries (row = query * group + head of the group) are the columns of the matrix
 // products, 16 * QT of them per workgroup, so that a key is read once for all of them.  Its waves take tiles of keys in
 // turn, each into its own two LDS buffers (no barrier until the end), and put their results together; a long text is cut
-// into spans of `span` tiles, one workgroup each, whose results window_join_kernel puts together.
+// into spans of `span` tiles, one workgroup each, whose results the last of them puts together, or window_join_kernel.
 // Bound by the bytes of the keys and values, 64 KB of them in flight per compute unit at head size 128: 16 tokens over 4000 to
-// 32768 kept rows of 8 heads in 0.19 ms, 5.1 TB/s (a large copy moves 4.7).  One token over a window of 1024: 9.6 us, of which
-// the two launches are half.
+// 32768 kept rows of 8 heads in 0.19 ms, 5.1 TB/s (a large copy moves 4.7).  One token over a window of 1024: 8.4 us, of which the
+// launch, the loads of the arguments and the queries, and joining the spans are three quarters.
 template <typename E, int D> struct FewImage {
     static constexpr int ROWB = D * (int)sizeof(E);
     static constexpr int PIECES = ROWB / 16;
@@ -505,9 +506,73 @@ struct FewArgs {
     bool by_seq;                     // a partial result's row: sequence * max_q + query instead of the query's row of q
     float2* part_ml;                 // [row][head][spans]: maximum, sum
     float* part_o;                   // [row][head][spans][D]
+    uint64_t* done;                  // [sequence][chunk][key/value head][spans]: `token` where the span's results are written; NULL:
+    uint64_t token;                  // window_join_kernel puts them together
 };
 __device__ __forceinline__ int64_t part_at(const WinArgs& a, const FewArgs& f, const Seq& sq, int seq, int j, int head) {
     return ((f.by_seq ? (int64_t)seq * a.max_q + j : sq.q0 + j) * a.hq + head) * f.spans;
+}
+
+// Values that workgroups on other XCDs read or wrote in the same launch: past the L2, which is an XCD's own.
+__device__ __forceinline__ void store_through(void* p, float x, float y) {
+    const uint64_t v = (uint64_t)__float_as_uint(y) << 32 | __float_as_uint(x);
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <bool THROUGH>
+__device__ __forceinline__ float2 load_pair(const void* p) {
+    if (!THROUGH) return *reinterpret_cast<const float2*>(p);
+    const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
+}
+
+// One wave: the results of n spans of a query row and head, in the order of the spans.
+template <typename E, int D, bool THROUGH>
+__device__ void join_row(const WinArgs& a, const FewArgs& f, const Seq& sq, int seq, int j, int head, int n, int lane) {
+    const int64_t at = part_at(a, f, sq, seq, j, head);
+    const float scale = fabsf(a.scale);
+    float top = NEG_BIG;
+    for (int i = lane; i < n; i += 64) top = fmaxf(top, load_pair<THROUGH>(f.part_ml + at + i).x);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    constexpr int DL = D / 4, PARTS = 64 / DL;               // four dimensions a lane, PARTS spans at a time
+    const int d = (lane % DL) * 4;
+    float total = 0.f;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    for (int i = lane / DL; i < n; i += 4 * PARTS) {         // (four spans' loads at once: one by one is a memory latency each)
+        float2 p[4], o0[4], o1[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int64_t from = at + min(i + u * PARTS, n - 1);
+            p[u] = load_pair<THROUGH>(f.part_ml + from);
+            o0[u] = load_pair<THROUGH>(f.part_o + from * D + d);
+            o1[u] = load_pair<THROUGH>(f.part_o + from * D + d + 2);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const float weight = i + u * PARTS < n ? __builtin_amdgcn_exp2f((p[u].x - top) * scale) : 0.f;
+            total += p[u].y * weight;
+            sum += f32x4{o0[u].x, o0[u].y, o1[u].x, o1[u].y} * weight;
+        }
+    }
+#pragma unroll
+    for (int o = DL; o < 64; o <<= 1) {
+        total += __shfl_xor(total, o, 64);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] += __shfl_xor(sum[e], o, 64);
+    }
+    const Seen w = seen_by(a, sq.nk - sq.nq + j, sq.nk);
+    const bool any_seen = w.s + (w.hi - w.lo) > 0;
+    const float inv = 1.f / total;
+    typename Vec<E, 4>::type v;
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float x = any_seen ? sum[e] * inv : 0.f;
+        bad |= x != x;
+        v[e] = (E)x;
+    }
+    if (__any(bad)) attend_row<E, D>(a, sq, j, head, lane);
+    else if (lane < DL) *reinterpret_cast<typename Vec<E, 4>::type*>(reinterpret_cast<E*>(a.out) + (sq.q0 + j) * a.out_stride + (int64_t)head * D + d) = v;
 }
 
 template <typename E, int D, int QT>
@@ -528,6 +593,7 @@ __global__ __launch_bounds__(64 * (FewImage<E, D>::NW)) void window_few_kernel(W
     const Tiles tiles = tiles_of(a, sq, j0, j1, KT);
     const int t0 = span * f.span, t1 = min(tiles.n, t0 + f.span);
     if (t0 >= t1 && span > 0) return;
+    const int spans = max(1, (tiles.n + f.span - 1) / f.span);          // that have keys
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -713,10 +779,11 @@ __global__ __launch_bounds__(64 * (FewImage<E, D>::NW)) void window_few_kernel(W
             total += p.y * weight;
             sum += *reinterpret_cast<const f32x4*>(sums + w * WAVE_F + lr * D + d) * weight;
         }
-        if (f.spans > 1) {
+        if (spans > 1) {
             const int64_t at = part_at(a, f, sq, seq, j, head) + span;
-            if (d == 0) f.part_ml[at] = make_float2(top, total);
-            *reinterpret_cast<f32x4*>(f.part_o + at * D + d) = sum;
+            if (d == 0) store_through(f.part_ml + at, top, total);
+            store_through(f.part_o + at * D + d, sum[0], sum[1]);
+            store_through(f.part_o + at * D + d + 2, sum[2], sum[3]);
         } else {
             const Seen w = seen_by(a, sq.nk - sq.nq + j, sq.nk);
             const bool any_seen = w.s + (w.hi - w.lo) > 0;
@@ -733,7 +800,33 @@ __global__ __launch_bounds__(64 * (FewImage<E, D>::NW)) void window_few_kernel(W
             *reinterpret_cast<typename Vec<E, 4>::type*>(reinterpret_cast<E*>(a.out) + (sq.q0 + j) * a.out_stride + (int64_t)head * D + d) = v;
         }
     }
-    if (f.spans > 1) return;
+    if (spans > 1) {
+        // The workgroup that finds the results of all spans written puts them together.  If two find it, both store the same values.  The
+        // marks may hold anything before the call: its token is none that an earlier call left, and they are cleared after use,
+        // so that a captured call finds them cleared when it runs again.
+        if (f.done == nullptr) return;
+        __shared__ int all;
+        uint64_t* done = f.done + ((int64_t)(seq * f.chunks + chunk) * a.hkv + kvh) * f.spans;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                // every thread's results are written, before ...
+        __syncthreads();
+        if (wave == 0) {
+            if (lane == 0) __hip_atomic_store(done + span, f.token, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");            // ... the mark, before the marks are read: the last one finds all
+            bool here = true;
+            for (int i = lane; i < spans; i += 64) here &= __hip_atomic_load(done + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == f.token;
+            const bool yes = __all(here);
+            if (yes)
+                for (int i = lane; i < spans; i += 64) __hip_atomic_store(done + i, (uint64_t)0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (lane == 0) all = yes;
+        }
+        __syncthreads();
+        if (!all) return;
+        for (int lr = wave; lr < rows; lr += NW) {
+            const int row = chunk * ROWS + lr;
+            join_row<E, D, true>(a, f, sq, seq, row / group, kvh * group + row % group, spans, lane);
+        }
+        return;
+    }
     __syncthreads();                                         // (also: the rows' stores are done before a row is written again)
     for (int lr = wave; lr < rows; lr += NW)
         if (bad_rows[lr >> 5] >> (lr & 31) & 1) {
@@ -742,9 +835,9 @@ __global__ __launch_bounds__(64 * (FewImage<E, D>::NW)) void window_few_kernel(W
         }
 }
 
-// The spans' results of one query row and head, a wave each.
+// The results of one query row and head whose chunks of rows are not put together by window_few_kernel, a wave each.
 template <typename E, int D>
-__global__ __launch_bounds__(256) void window_join_kernel(WinArgs a, FewArgs f, int rows_of_chunk, uint32_t* fault) {
+__global__ __launch_bounds__(256) void window_join_kernel(WinArgs a, FewArgs f, int rows_of_chunk) {
     const int group = a.hq / a.hkv, lane = threadIdx.x & 63;
     const int per_seq = (a.max_q * a.hq + 3) / 4;
     const int seq = (int)(blockIdx.x / per_seq);
@@ -755,42 +848,8 @@ __global__ __launch_bounds__(256) void window_join_kernel(WinArgs a, FewArgs f, 
     const int chunk = (j * group + head % group) / rows_of_chunk;
     const int last = min((chunk + 1) * rows_of_chunk, sq.nq * group) - 1;
     const Tiles tiles = tiles_of(a, sq, chunk * rows_of_chunk / group, last / group, FewImage<E, D>::KT);
-    const int n = max(1, (tiles.n + f.span - 1) / f.span);
-    const int64_t at = part_at(a, f, sq, seq, j, head);
-    const float scale = fabsf(a.scale);
-    float top = NEG_BIG;
-    for (int i = lane; i < n; i += 64) top = fmaxf(top, f.part_ml[at + i].x);
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-    constexpr int DL = D / 4, PARTS = 64 / DL;               // four dimensions a lane, PARTS spans at a time
-    const int d = (lane % DL) * 4;
-    float total = 0.f;
-    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-    for (int i = lane / DL; i < n; i += PARTS) {
-        const float2 p = f.part_ml[at + i];
-        const float weight = __builtin_amdgcn_exp2f((p.x - top) * scale);
-        total += p.y * weight;
-        sum += *reinterpret_cast<const f32x4*>(f.part_o + (at + i) * D + d) * weight;
-    }
-#pragma unroll
-    for (int o = DL; o < 64; o <<= 1) {
-        total += __shfl_xor(total, o, 64);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sum[e] += __shfl_xor(sum[e], o, 64);
-    }
-    const Seen w = seen_by(a, sq.nk - sq.nq + j, sq.nk);
-    const bool any_seen = w.s + (w.hi - w.lo) > 0;
-    const float inv = 1.f / total;
-    typename Vec<E, 4>::type v;
-    bool bad = false;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const float x = any_seen ? sum[e] * inv : 0.f;
-        bad |= x != x;
-        v[e] = (E)x;
-    }
-    if (__any(bad)) attend_row<E, D>(a, sq, j, head, lane);
-    else if (lane < DL) *reinterpret_cast<typename Vec<E, 4>::type*>(reinterpret_cast<E*>(a.out) + (sq.q0 + j) * a.out_stride + (int64_t)head * D + d) = v;
+    const int n = (tiles.n + f.span - 1) / f.span;
+    if (n > 1) join_row<E, D, false>(a, f, sq, seq, j, head, n, lane);          // (one span's results are stored as they are)
 }
 
 // How a call runs, from its sizes alone (the workspace is computed from the same).
@@ -798,6 +857,8 @@ struct Plan {
     bool few;
     int qt, chunks, spans, span;     // few: 16-row columns of a workgroup, its row chunks, spans along the keys
     int64_t parts;                   // query rows * heads * spans whose partial results the workspace holds
+    int64_t marks;                   // 0: window_join_kernel puts them together
+    int64_t bytes(int D) const { return marks * 8 + parts * (D + 2) * 4; }
 };
 
 // The most keys that `queries` neighbouring queries can see, in tiles of kt
@@ -836,14 +897,21 @@ Plan plan_of(int64_t total_q, int n_seq, int max_q, int max_k, int hq, int hkv, 
     // A workgroup's start, the filling of its buffers and its end cost as much as some 8 tiles a wave, so the workgroups that are on
     // the chip at once (256 compute units by what their LDS leaves room for) run one round: one token over 32768 keys of 8 heads
     // 36.6 us, in two rounds 44, in three 51.  Spans that would be long all the same (over 256 tiles) are cut in three, against
-    // sequences of unlike lengths: 16 sequences of 4000 to 32768 keys 223 -> 190 us.  Below 8 tiles a span, or 20 in all,
-    // joining costs more than it gives (window 1024: spans of 16 tiles 11.5 us, 8: 10.0; 512 keys: one span 8.2 us, two 9.3).
+    // sequences of unlike lengths: 16 sequences of 4000 to 32768 keys 223 -> 190 us.  Spans of 4 tiles, a wave's one, are the
+    // shortest while they are few, 8 from 128 tiles on (one token, head size 128: 1024 keys in spans of 4 7.6 us, 8 8.6, 12 9.6; 4096
+    // keys 9.8, 9.2, 10.6).  One span, where joining costs more than it gives, by what its tiles take (512 keys: one span 8.1
+    // us, spans of 4 7.8, at head size 64 6.4 and 6.8; 200 keys in float32: 10.5 and 8.4).
     const int64_t on_chip = 256 * ((160 << 10) / (16 * (int64_t)kt * D * size + 2048));
     int64_t cuts = std::max<int64_t>(1, on_chip / base);
     if (tiles / cuts > 256) cuts = std::max<int64_t>(1, 3 * on_chip / base);
-    p.span = (int)(tiles <= 20 ? tiles : std::max<int64_t>(8, (tiles + cuts - 1) / cuts));
+    const int64_t one_span = std::min(20, (wide ? 768 : 2048) / D), shortest = std::min<int64_t>(8, std::max<int64_t>(4, tiles / 16));
+    p.span = (int)(tiles <= one_span ? tiles : std::max(shortest, (tiles + cuts - 1) / cuts));
     p.spans = (int)((tiles + p.span - 1) / p.span);
     p.parts = p.spans > 1 ? std::min(total_q, (int64_t)n_seq * max_q) * hq * p.spans : 0;
+    // Joined by the workgroups themselves, a row each wave, where that is the shorter (one token of 4 heads on one, head size 128:
+    // 1024 keys 8.8 us, with the second launch 9.4; 65536 keys, 256 spans, 28.5 and 26.1; 8 rows on 1024 keys 10.6 and 9.8) or saves
+    // a launch of the host's 4 us at no more than 6 % (16384 keys, 64 spans: 13.0 us and 12.3).
+    if (p.spans > 1 && rows <= 4 && p.spans <= 64) p.marks = ((int64_t)n_seq * p.chunks * hkv * p.spans + 1) / 2 * 2;
     return p;
 }
 
@@ -852,7 +920,10 @@ int window_few(const WinArgs& a, const Plan& p, void* work, hipStream_t stream) 
     FewArgs f;
     f.chunks = p.chunks; f.spans = p.spans; f.span = p.span;
     f.by_seq = (int64_t)a.n_seq * a.max_q < a.total_q;       // rows of no sequence take no room
-    f.part_o = reinterpret_cast<float*>(work);
+    static std::atomic<uint64_t> tokens{(uint64_t)std::chrono::steady_clock::now().time_since_epoch().count() * 0x9e3779b97f4a7c15ull | 1};
+    f.done = p.marks > 0 ? reinterpret_cast<uint64_t*>(work) : nullptr;
+    f.token = p.marks > 0 ? tokens.fetch_add(2) : 0;         // (odd: never what a call leaves)
+    f.part_o = reinterpret_cast<float*>(reinterpret_cast<uint64_t*>(work) + p.marks);
     f.part_ml = reinterpret_cast<float2*>(f.part_o + p.parts * D);
     const int64_t grid = (int64_t)a.n_seq * p.spans * p.chunks * a.hkv;
     RAG_REQUIRE(grid < (1ll << 31), RAG_ELIMIT, "rag_enc_attention_window: too many sequences");
@@ -860,10 +931,10 @@ int window_few(const WinArgs& a, const Plan& p, void* work, hipStream_t stream) 
     RAG_GRANT_LDS((window_few_kernel<T, D, QT>), lds);
     window_few_kernel<T, D, QT><<<(unsigned)grid, 64 * FewImage<T, D>::NW, lds, stream>>>(a, f, rag_fault_word());
     RAG_HIP_TRY(hipGetLastError());
-    if (p.spans > 1) {
+    if (p.spans > 1 && p.marks == 0) {
         const int64_t joins = (int64_t)a.n_seq * (((int64_t)a.max_q * a.hq + 3) / 4);
         RAG_REQUIRE(joins < (1ll << 31), RAG_ELIMIT, "rag_enc_attention_window: too many query rows");
-        window_join_kernel<T, D><<<(unsigned)joins, 256, 0, stream>>>(a, f, 16 * QT, rag_fault_word());
+        window_join_kernel<T, D><<<(unsigned)joins, 256, 0, stream>>>(a, f, 16 * QT);
         RAG_HIP_TRY(hipGetLastError());
     }
     return RAG_OK;
@@ -873,8 +944,8 @@ template <typename T, int D>
 int window_launch(const WinArgs& a, void* work, int64_t work_bytes, hipStream_t stream) {
     const Plan p = plan_of(a.total_q, a.n_seq, a.max_q, a.max_k, a.hq, a.hkv, D, a.left, a.right, a.sinks, (int)sizeof(T));
     if (p.few) {
-        RAG_REQUIRE(p.parts * (D + 2) * 4 <= work_bytes, RAG_EINVAL, "rag_enc_attention_window: the workspace holds %lld bytes, %lld are needed",
-                    (long long)work_bytes, (long long)(p.parts * (D + 2) * 4));
+        RAG_REQUIRE(p.bytes(D) <= work_bytes, RAG_EINVAL, "rag_enc_attention_window: the workspace holds %lld bytes, %lld are needed",
+                    (long long)work_bytes, (long long)p.bytes(D));
         if (p.qt == 1) return window_few<T, D, 1>(a, p, work, stream);
         if (p.qt == 2) return window_few<T, D, 2>(a, p, work, stream);
         return window_few<T, D, 4>(a, p, work, stream);
@@ -910,7 +981,7 @@ extern "C" int64_t rag_enc_attention_window_workspace(int64_t total_q, int32_t n
         return 0;                                            // nothing to run, or refused by the call
     const Plan p = plan_of(total_q, n_seq, max_q_len, max_k_len, n_q_heads, n_kv_heads, head_dim, window_left >= FAR ? -1 : window_left,
                            window_right >= FAR ? -1 : window_right, n_sinks, dtype == RAG_DTYPE_F32 ? 4 : 2);
-    return p.parts * (head_dim + 2) * 4;
+    return p.bytes(head_dim);
 }
 
 extern "C" int rag_enc_attention_window_dev(const void* d_q, int64_t q_stride, const void* d_k, int64_t k_row_stride,

@@ -400,3 +400,95 @@ def test_a_layer_of_all_three_token_by_token_and_at_once():
     for got in runs:
         assert bool(((got - want).abs() <= tol).all())
         assert float((got - want).pow(2).mean().sqrt()) <= 0.1 * float(tol.pow(2).mean().sqrt())
+
+
+@pytest.mark.parametrize('kind', list(TYPES))
+def test_a_workspace_may_hold_anything(kind):
+    # Spans' results are put together by the workgroups of the call itself, which mark what they have written in the workspace.
+    # Whatever the memory holds, the same call gives the same bits: zeros, ones, what another call of other sizes
+    # left there, what this call left there, and a captured call that finds its own leavings when it is replayed.
+    import rag_hip
+    dt, dev, hq, hkv, d = TYPES[kind], _dev(), 4, 2, 64
+    code = {'f32': 0, 'bf16': 1, 'f16': 2}[kind]
+    lens = [1500, 0, 3, 2600, 40, 700, 2599]
+    g = _gen(91)
+    k = torch.randn((sum(lens), hkv, d), generator=g, device=dev).to(dt)
+    v = torch.randn((sum(lens), hkv, d), generator=g, device=dev).to(dt)
+    q = torch.randn((len(lens), hq, d), generator=g, device=dev).to(dt)
+    ks = [sum(lens[:i]) for i in range(len(lens))]
+    cu, k_start = _cu([1] * len(lens)), torch.tensor(ks, dtype=torch.int64, device=dev)
+    k_len = torch.tensor(lens, dtype=torch.int32, device=dev)
+    lib = rag_hip.load_library()
+    work = torch.zeros((1 << 20,), dtype=torch.uint8, device=dev)
+
+    def call(left, out):
+        need = lib.rag_enc_attention_window_workspace(len(lens), len(lens), 1, 2600, hq, hkv, d, left, 0, 2, code)
+        assert 0 < need <= work.numel()
+        rc = lib.rag_enc_attention_window_dev(q.data_ptr(), hq * d, k.data_ptr(), hkv * d, d, v.data_ptr(), hkv * d, d, cu.data_ptr(), len(lens),
+                                              k_start.data_ptr(), k_len.data_ptr(), sum(lens), len(lens), 1, 2600, hq, hkv, d, d ** -0.5, left, 0, 2,
+                                              code, out.data_ptr(), hq * d, work.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+        return out
+
+    def fresh():
+        return torch.full((len(lens), hq * d), 7.0, dtype=dt, device=dev)
+
+    want = {left: call(left, fresh()) for left in (-1, 1400)}
+    for left in (-1, 1400):
+        _check(want[left], q, k, v, [1] * len(lens), list(zip(ks, lens)), left, 0, 2, d ** -0.5)
+    for fill in (0, 0xff, None):
+        for left in (-1, 1400, -1):
+            if fill is not None:
+                work.fill_(fill)
+            assert torch.equal(call(left, fresh()), want[left])
+    out = fresh()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=side):
+        call(-1, out)
+    for i in range(6):
+        out.fill_(3.0)
+        graph.replay()
+        assert torch.equal(out, want[-1]), i
+        assert torch.equal(call(1400, fresh()), want[1400])
+        torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize('kind', list(TYPES))
+@pytest.mark.parametrize('hq,hkv', [(4, 1), (16, 1)])
+def test_many_spans(kind, hq, hkv):
+    # one token whose keys are cut into few spans and into many, a length that ends inside a tile and a span, and one key
+    import rag_hip
+    dt, dev, d = TYPES[kind], _dev(), 64
+    for nk, max_k in ((1, 20000), (33, 20000), (1029, 1029), (5003, 20000), (20000, 20000), (30011, 30011)):
+        g = _gen(nk)
+        k, v = (torch.randn((nk, hkv, d), generator=g, device=dev).to(dt) for _ in range(2))
+        q = torch.randn((1, hq, d), generator=g, device=dev).to(dt)
+        got = rag_hip.enc_attention_window_dev(q, k, v, _cu([1]), 1, k_start=torch.zeros(1, dtype=torch.int64, device=dev),
+                                               k_len=torch.full((1,), nk, dtype=torch.int32, device=dev), max_k_len=max_k, window_right=0)
+        _check(got, q, k, v, [1], [(0, nk)], -1, 0, 0, d ** -0.5)
+
+
+def test_two_streams_at_once():
+    # two calls whose spans are on the chip together, each with its own workspace
+    import rag_hip
+    dt, dev, hq, hkv, d, nk = torch.bfloat16, _dev(), 4, 1, 128, 6000
+    g = _gen(17)
+    k, v = (torch.randn((2 * nk, hkv, d), generator=g, device=dev).to(dt) for _ in range(2))
+    q = torch.randn((2, hq, d), generator=g, device=dev).to(dt)
+    one, cu = torch.full((1,), nk, dtype=torch.int32, device=dev), _cu([1])
+    starts = [torch.full((1,), i * nk, dtype=torch.int64, device=dev) for i in range(2)]
+
+    def call(i):
+        return rag_hip.enc_attention_window_dev(q[i:i + 1], k, v, cu, 1, k_start=starts[i], k_len=one, max_k_len=nk, window_right=0)
+
+    want = [call(i) for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(call(i))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want[i]) for i in range(2) for x in got[i])
