@@ -56,7 +56,7 @@ def test_workspace_goes_by_the_sizes_and_never_overflows():
     import rag_hip
     f = rag_hip.load_library().rag_enc_attention_window_workspace
     one = f(1, 1, 1, 32768, 32, 8, 128, -1, 0, 0, 1)
-    assert one > 0 and one % (32 * 130 * 4) == 0               # spans of one token's 32 heads: 128 sums, a maximum and a total
+    assert one > 0 and one % (32 * 130 * 4 + 8 * 8) == 0       # spans of one token's 32 heads: 128 sums, a maximum and a total; a mark of each key head
     assert f(1 << 30, 1, 1, 32768, 32, 8, 128, -1, 0, 0, 1) == one       # rows of no sequence take no room
     assert f(16384, 1, 16384, 16384, 16, 8, 128, 4096, 0, 4, 1) == 0 and f(0, 0, 0, 0, 1, 1, 64, -1, -1, 0, 0) == 0
     big = (1 << 31) - 1
