@@ -11,6 +11,7 @@
 #include <algorithm>
 #include <atomic>
 #include <chrono>
+#include <type_traits>
 
 #include <math.h>
 
@@ -149,27 +150,56 @@ __device__ __forceinline__ void lds_dma16(uint32_t lds_dst, const void* gbase, u
                  : "=&s"(keep) : "v"(voff), "s"(lds_dst), "s"(gbase) : "memory");
 }
 
-// The image of a tile of keys or values in LDS: rows of D elements, the 16-byte piece p of row `key` at place
+// 16 neighbouring rows of `pieces` 16-byte pieces, piece p of a row at place p ^ swizzle, cover all banks once at one p
+__device__ __forceinline__ int rows_swizzle(int pieces, int row) {
+    return pieces >= 16 ? row & 15 : pieces == 8 ? (row >> 1) & 7 : (row >> 2) & 3;
+}
+
+// The image of a tile of keys or values in LDS: rows of D 16-bit elements, the 16-byte piece p of row `key` at place
 // p ^ swizzle(key), so that neither the rows that a matrix operand reads at one piece nor the blocks that the
-// transposing read takes fall on the same banks.
+// transposing read takes fall on the same banks.  fp32: three such images, of the first, second and third 8 bits of the values.
 template <typename E, int D> struct Image {
-    static constexpr int ROWB = D * (int)sizeof(E);          // bytes of a row
+    static constexpr int PARTS = sizeof(E) == 4 ? 3 : 1;
+    static constexpr int ROWB = D * 2;                       // bytes of a row
     static constexpr int PIECES = ROWB / 16;
     static constexpr int KT = sizeof(E) == 4 ? 32 : 64;      // keys of a tile
-    static constexpr int BYTES = KT * ROWB;
+    static constexpr int PART = KT * ROWB;
+    static constexpr int BYTES = PARTS * PART;
     // tiles in LDS at a time: what the registers' occupancy leaves room for
-    static constexpr int BUFFERS = BYTES > 4096 ? 2 : 4;
-    static constexpr int WAVES = sizeof(E) == 4 ? (D == 128 ? 1 : D == 64 ? 2 : 4) : (D == 128 ? 2 : D == 64 ? 3 : 4);        // per SIMD
-    // 16 neighbouring rows at one piece index cover all banks once
-    __device__ static int k_swizzle(int row) {
-        return PIECES >= 16 ? row & 15 : PIECES == 8 ? (row >> 1) & 7 : (row >> 2) & 3;
-    }
-    // 16 bits: 4 neighbouring rows x 4 neighbouring pieces; 32 bits: rows 4 apart, 8 pieces
+    static constexpr int BUFFERS = sizeof(E) == 4 ? (D == 128 ? 1 : 2) : D == 32 ? 4 : 2;
+    static constexpr int WAVES = sizeof(E) == 4 ? (D == 128 ? 2 : D == 64 ? 3 : 4) : (D == 128 ? 2 : D == 64 ? 3 : 4);        // per SIMD
+    __device__ static int k_swizzle(int row) { return rows_swizzle(PIECES, row); }
+    // 4 neighbouring rows x 4 neighbouring pieces
     __device__ static int v_swizzle(int row) {
-        if (sizeof(E) == 4) return PIECES >= 16 ? ((row >> 2) & 1) << 3 : 0;
         return PIECES == 16 ? (row & 3) << 2 | ((row >> 2) & 3) : PIECES == 8 ? ((row >> 1) & 1) << 2 | ((row >> 2) & 3) : 0;
     }
 };
+
+// Two fp32 values as three pairs of bf16, x = x0 + x1 + x2 exactly (8 significant bits each, the rest of every cut is exact)
+__device__ __forceinline__ void split_pair(float x, float y, uint32_t& w0, uint32_t& w1, uint32_t& w2) {
+    const auto cut = [](float v) { return __uint_as_float(__float_as_uint(v) & 0xffff0000u); };
+    const auto high = [](float a, float b) { return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u); };
+    const float x1 = x - cut(x), y1 = y - cut(y);
+    w0 = high(x, y);
+    w1 = high(x1, y1);
+    w2 = high(x1 - cut(x1), y1 - cut(y1));
+}
+template <int PARTS, typename V>
+__device__ __forceinline__ void split8(const float* v, V* parts) {
+    uint32_t w[3][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) split_pair(v[2 * i], v[2 * i + 1], w[0][i], w[1][i], w[2][i]);
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) parts[p] = V{w[p][0], w[p][1], w[p][2], w[p][3]};
+}
+// The products of three parts that reach 24 bits, the small ones first
+template <typename M, typename F, typename V>
+__device__ __forceinline__ F product(const V* x, const V* y, F c) {
+    typedef typename M::x8 x8;
+    const auto mul = [&](int i, int j) { c = M::mfma(__builtin_bit_cast(x8, x[i]), __builtin_bit_cast(x8, y[j]), c); };
+    mul(2, 0); mul(0, 2); mul(1, 1); mul(1, 0); mul(0, 1); mul(0, 0);
+    return c;
+}
 
 template <typename E> struct Mma;
 template <> struct Mma<bf16> {
@@ -205,7 +235,8 @@ constexpr float LAG = 8.f;           // the maximum may lag behind by this power
 template <typename E, int D>
 __global__ __launch_bounds__(256, (Image<E, D>::WAVES)) void window_tile_kernel(WinArgs a, int q_tiles, uint32_t units, bool by_pair, uint32_t* fault) {
     typedef Image<E, D> I;
-    constexpr int KT = I::KT, KB = KT / 32, DT = D / 32, KC = I::PIECES / 2, NB = I::BUFFERS;
+    typedef typename std::conditional<sizeof(E) == 4, bf16, E>::type M;          // of the matrix operands
+    constexpr int KT = I::KT, KB = KT / 32, DT = D / 32, KC = I::PIECES / 2, NB = I::BUFFERS, PARTS = I::PARTS;
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
     // All units of a (sequence, key/value head) pair go to workgroups with the same blockIdx % 8, which round-robin
@@ -265,26 +296,83 @@ __global__ __launch_bounds__(256, (Image<E, D>::WAVES)) void window_tile_kernel(
             lds_dma16(dst + I::BYTES + n * 1024, vp, src * v_rowb + (place ^ I::v_swizzle(row)) * 16);
         }
     };
-    if (n_tiles > 0) stage(0);
+    // fp32: rows into registers, from there as three parts into LDS
+    constexpr int LOADS = PARTS == 3 ? 2 * KT * I::PIECES / 256 : 1;
+    float raw[LOADS][8];
+    auto place_of = [&](int j, bool& value, int& row, int& piece) {
+        const int n = tid + 256 * j;
+        value = n >= KT * I::PIECES;
+        row = n / I::PIECES % KT;
+        piece = n % I::PIECES;
+    };
+    auto fetch = [&](int t) {
+        const int key0 = first_key(t);
+        const int last = sq.nk - 1 - key0;
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) {
+            bool value;
+            int row, piece;
+            place_of(j, value, row, piece);
+            const unsigned char* p = (value ? vbase : kbase) + (int64_t)key0 * (value ? v_rowb : k_rowb) + (uint32_t)min(row, last) * (value ? v_rowb : k_rowb) + piece * 32;
+            const float4 x = reinterpret_cast<const float4*>(p)[0], y = reinterpret_cast<const float4*>(p)[1];
+            raw[j][0] = x.x; raw[j][1] = x.y; raw[j][2] = x.z; raw[j][3] = x.w;
+            raw[j][4] = y.x; raw[j][5] = y.y; raw[j][6] = y.z; raw[j][7] = y.w;
+        }
+    };
+    auto put = [&](int t) {
+        unsigned char* dst = smem + (t % NB) * 2 * I::BYTES;
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) {
+            bool value;
+            int row, piece;
+            place_of(j, value, row, piece);
+            u32x4 w[3];
+            split8<3>(raw[j], w);
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p)
+                *reinterpret_cast<u32x4*>(dst + (value ? I::BYTES : 0) + p * I::PART + row * I::ROWB + (piece ^ (value ? I::v_swizzle(row) : I::k_swizzle(row))) * 16) = w[p];
+        }
+    };
+    if (n_tiles > 0) {
+        if constexpr (PARTS == 1) stage(0);
+        else fetch(0);
+    }
 
     // Q^T: piece 2c + h of the lane's query
     const bool flip = a.scale < 0.f;                         // a negative scale goes into q: the maximum is taken of products as they are
     const float scale = fabsf(a.scale);
-    u32x4 qf[KC];
+    u32x4 qf[KC][PARTS];
     {
         const unsigned char* qp = reinterpret_cast<const unsigned char*>(a.q) + ((sq.q0 + min(qr, sq.nq - 1)) * a.q_stride + (int64_t)head * D) * (int64_t)sizeof(E);
 #pragma unroll
         for (int c = 0; c < KC; ++c) {
-            qf[c] = *reinterpret_cast<const u32x4*>(qp + (2 * c + h) * 16);
-            if (flip) qf[c] ^= sizeof(E) == 4 ? 0x80000000u : 0x80008000u;
+            if constexpr (PARTS == 1) {
+                qf[c][0] = *reinterpret_cast<const u32x4*>(qp + (2 * c + h) * 16);
+                if (flip) qf[c][0] ^= 0x80008000u;
+            } else {
+                float v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    v[i] = reinterpret_cast<const float*>(qp)[(2 * c + h) * 8 + i];
+                    if (flip) v[i] = -v[i];
+                }
+                split8<PARTS>(v, qf[c]);
+            }
         }
     }
     // (the queries, the last loads so far, are waited for here: later their wait would cover the tiles behind the first too)
 #pragma unroll
-    for (int c = 0; c < KC; ++c) asm volatile("" : "+v"(qf[c]));
+    for (int c = 0; c < KC; ++c)
 #pragma unroll
-    for (int t = 1; t < NB - 1; ++t)
-        if (t < n_tiles) stage(t);
+        for (int p = 0; p < PARTS; ++p) asm volatile("" : "+v"(qf[c][p]));
+    if constexpr (PARTS == 1) {
+#pragma unroll
+        for (int t = 1; t < NB - 1; ++t)
+            if (t < n_tiles) stage(t);
+    } else if (NB == 2 && n_tiles > 0) {
+        put(0);
+        if (n_tiles > 1) fetch(1);
+    }
     float m_run = NEG_BIG, l_run = 0.f;                      // l_run: the lane's own keys
     f32x16 o[DT];
 #pragma unroll
@@ -293,12 +381,26 @@ __global__ __launch_bounds__(256, (Image<E, D>::WAVES)) void window_tile_kernel(
         for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
 
     for (int t = 0; t < n_tiles; ++t) {
-        // this tile's loads; those of the next NB - 2 stay in flight
-        if (NB > 2 && t + NB - 2 < n_tiles) asm volatile("s_waitcnt vmcnt(%0)" :: "n"((NB - 2) * (I::BYTES / 2048)) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();                        // every wave has its part, and is done with the tile before
-        asm volatile("" ::: "memory");
-        if (t + NB - 1 < n_tiles) stage(t + NB - 1);
+        if constexpr (PARTS == 1) {
+            // this tile's loads; those of the next NB - 2 stay in flight
+            if (NB > 2 && t + NB - 2 < n_tiles) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"((NB - 2) * (I::BYTES / 2048)) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();                    // every wave has its part, and is done with the tile before
+            asm volatile("" ::: "memory");
+            if (t + NB - 1 < n_tiles) stage(t + NB - 1);
+        } else {
+            if (NB == 1) {
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                __builtin_amdgcn_s_barrier();                // every wave is done with the tile before
+                asm volatile("" ::: "memory");
+                put(t);
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();                    // the tile is there
+            asm volatile("" ::: "memory");
+            if (NB == 2 && t + 1 < n_tiles) put(t + 1);
+            if (t + NB < n_tiles) fetch(t + NB);
+        }
         const int key0 = first_key(t);
         // whether some query of the wave sees some of the tile, and whether all see all of it
         const bool some = wave_on && key0 < w_last.hi && (key0 + KT > w_first.lo || key0 < a.sinks);
@@ -315,14 +417,12 @@ __global__ __launch_bounds__(256, (Image<E, D>::WAVES)) void window_tile_kernel(
         for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
             for (int c = 0; c < KC; ++c) {
-                const u32x4 kf = *reinterpret_cast<const u32x4*>(ks + (kb * 32 + r) * I::ROWB + ((2 * c + h) ^ I::k_swizzle(r)) * 16);
-                if constexpr (sizeof(E) == 4) {
+                u32x4 kf[PARTS];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        s[kb] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kf[j]), __uint_as_float(qf[c][j]), s[kb], 0, 0, 0);
-                } else {
-                    s[kb] = Mma<E>::mfma(__builtin_bit_cast(typename Mma<E>::x8, kf), __builtin_bit_cast(typename Mma<E>::x8, qf[c]), s[kb]);
-                }
+                for (int p = 0; p < PARTS; ++p)
+                    kf[p] = *reinterpret_cast<const u32x4*>(ks + p * I::PART + (kb * 32 + r) * I::ROWB + ((2 * c + h) ^ I::k_swizzle(r)) * 16);
+                if constexpr (PARTS == 1) s[kb] = Mma<M>::mfma(__builtin_bit_cast(typename Mma<M>::x8, kf[0]), __builtin_bit_cast(typename Mma<M>::x8, qf[c][0]), s[kb]);
+                else s[kb] = product<Mma<M>>(kf, qf[c], s[kb]);
             }
         }
         if (!whole) {
@@ -364,34 +464,38 @@ __global__ __launch_bounds__(256, (Image<E, D>::WAVES)) void window_tile_kernel(
             }
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
-            if constexpr (sizeof(E) == 4) {
+            typedef short tr4 __attribute__((__vector_size__(4 * sizeof(short))));
+            const int rho = (lane & 15) >> 2, col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
+            for (int tt = 0; tt < 2; ++tt) {
+                u32x4 pb[PARTS];
+                if constexpr (PARTS == 1) {
+                    typename Mma<M>::x8 x;
 #pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) {
-                        const int key = 32 * kb + 8 * (i >> 2) + 4 * h + (i & 3);
-                        const float v = *reinterpret_cast<const float*>(vs + key * I::ROWB + ((dt * 8 + (r >> 2)) ^ I::v_swizzle(key)) * 16 + (r & 3) * 4);
-                        o[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, s[kb][i], o[dt], 0, 0, 0);
-                    }
-            } else {
-                typedef short tr4 __attribute__((__vector_size__(4 * sizeof(short))));
-                const int rho = (lane & 15) >> 2, col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+                    for (int j = 0; j < 8; ++j) x[j] = (M)s[kb][8 * tt + j];
+                    pb[0] = __builtin_bit_cast(u32x4, x);
+                } else {
+                    float v[8];
 #pragma unroll
-                for (int tt = 0; tt < 2; ++tt) {
-                    typename Mma<E>::x8 pb;
+                    for (int j = 0; j < 8; ++j) v[j] = s[kb][8 * tt + j];
+                    split8<PARTS>(v, pb);
+                }
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) pb[j] = (E)s[kb][8 * tt + j];
+                for (int dt = 0; dt < DT; ++dt) {
+                    union { tr4 t[2]; u32x4 v; } av[PARTS];
+                    u32x4 vf[PARTS];
 #pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) {
-                        union { tr4 t[2]; typename Mma<E>::x8 v; } av;
+                    for (int p = 0; p < PARTS; ++p) {
 #pragma unroll
                         for (int u = 0; u < 2; ++u) {
                             const int row = 32 * kb + 16 * tt + 8 * u + 4 * h + rho;
-                            const unsigned char* p = vs + row * I::ROWB + ((dt * 4 + (col >> 3)) ^ I::v_swizzle(row)) * 16 + (col & 4) * 2;
-                            av.t[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) tr4*)p);
+                            const unsigned char* at = vs + p * I::PART + row * I::ROWB + ((dt * 4 + (col >> 3)) ^ I::v_swizzle(row)) * 16 + (col & 4) * 2;
+                            av[p].t[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) tr4*)at);
                         }
-                        o[dt] = Mma<E>::mfma(av.v, pb, o[dt]);
+                        vf[p] = av[p].v;
                     }
+                    if constexpr (PARTS == 1) o[dt] = Mma<M>::mfma(__builtin_bit_cast(typename Mma<M>::x8, vf[0]), __builtin_bit_cast(typename Mma<M>::x8, pb[0]), o[dt]);
+                    else o[dt] = product<Mma<M>>(vf, pb, o[dt]);
                 }
             }
         }
@@ -457,7 +561,7 @@ template <typename E, int D> struct FewImage {
     static constexpr int BYTES = KT * ROWB;
     static constexpr int NW = 4;                             // waves
     static constexpr size_t lds(int rows) { return (size_t)NW * (4 * BYTES + rows * 8); }
-    __device__ static int k_swizzle(int row) { return Image<E, D>::k_swizzle(row); }
+    __device__ static int k_swizzle(int row) { return rows_swizzle(PIECES, row); }
     // 16 bits: 8 neighbouring rows x 2 neighbouring pieces; 32 bits: rows 4 apart, 4 pieces
     __device__ static int v_swizzle(int row) {
         if (sizeof(E) == 4) return PIECES >= 16 ? ((row >> 2) & 3) << 2 : ((row >> 2) & 1) << 2;
