@@ -166,8 +166,8 @@ template <typename E, int D> struct Image {
     static constexpr int PART = KT * ROWB;
     static constexpr int BYTES = PARTS * PART;
     // tiles in LDS at a time: what the registers' occupancy leaves room for
-    static constexpr int BUFFERS = sizeof(E) == 4 ? (D == 128 ? 1 : 2) : D == 32 ? 4 : 2;
-    static constexpr int WAVES = sizeof(E) == 4 ? (D == 128 ? 2 : D == 64 ? 3 : 4) : (D == 128 ? 2 : D == 64 ? 3 : 4);        // per SIMD
+    static constexpr int BUFFERS = sizeof(E) == 4 ? (D == 32 ? 1 : 2) : D == 32 ? 4 : 2;
+    static constexpr int WAVES = sizeof(E) == 4 ? (D == 128 ? 1 : D == 64 ? 2 : 4) : (D == 128 ? 2 : D == 64 ? 3 : 4);        // per SIMD
     __device__ static int k_swizzle(int row) { return rows_swizzle(PIECES, row); }
     // 4 neighbouring rows x 4 neighbouring pieces
     __device__ static int v_swizzle(int row) {
@@ -218,20 +218,25 @@ constexpr float NEG_BIG = -1e30f;    // the running maximum's start: finite, so 
 constexpr float LAG = 8.f;           // the maximum may lag behind by this power of two before the sums are rescaled
 
 // Four waves, each 32 queries (the columns of the matrix products) of a 128-query tile of one head; tiles of keys and values
-// come into LDS by direct loads into a ring of two to four, the next tiles' loads in flight while this one is worked on, one barrier a tile.
+// come into LDS, the next tiles' loads in flight while this one is worked on: 16 bits by direct loads into a ring of two to four,
+// fp32 through registers, where they are cut into parts; one barrier a tile (fp32 at head size 32: one buffer, two).
 //   S^T = K Q^T        rows = keys, a lane holds 16 keys (registers, lane half) of its query (lane % 32)
 //   O^T += V^T P^T     the lane's probabilities are the B operand as they stand; V^T comes out of the row-major image
-//                      through the transposing LDS read (16 bits) or by single values (fp32)
+//                      through the transposing LDS read
 // 16-bit types: probabilities are rounded to the type (half a step of each; the result is as far from the exact one again as
-// its own rounding takes it), their sum and all other sums are fp32.  fp32: v_mfma_f32_32x32x2_f32, exact fp32 products.
+// its own rounding takes it), their sum and all other sums are fp32.
+// fp32: queries, keys, values and probabilities as sums of three bf16 each, exactly; of the nine products the six that reach
+// 2^-20 of the factors are taken (the other three stay below 2^-20 together, an fp32 sum over 32 dimensions may be off by 2^-19), all in fp32.
+// The matrix cores do six bf16 products in 3/8 of the time of an fp32 one: 4096 tokens, causal, 16 heads of 128 on 8: 411 us,
+// with fp32 products 602; 40 sequences of 1 to 512 tokens, 12 heads of 32, window 128: 35.5 and 58.
 // The running maximum is raised only when a score exceeds it by more than LAG (the probabilities stay below 2^LAG, in
 // the range of every type), so that the rescaling of the sums is rare.
 // Masked scores are -infinity; a tile that every query of the wave sees whole needs no mask, one that none sees is left
 // out.  Where keys or values hold infinities or NaN, 0 * infinity spoils rows that do not see them: every row that ends as
 // NaN is computed again by attend_row, which reads only what the row sees.
 // Bound by the matrix cores and the exponentials together: 16384 tokens, 16 heads of 128 on 8, window 4096: 0.48-0.50 ms,
-// 0.97-1.0 PFLOP/s (a library product of 8192^3 reaches 1.2); head size 64, no window: 0.36 ms for 2 x 8192, 0.77; float32 at
-// 128: 114 TFLOP/s of the 153 of a library product.
+// 0.97-1.0 PFLOP/s (a library product of 8192^3 reaches 1.2); head size 64, no window: 0.36 ms for 2 x 8192, 0.77; float32:
+// 167 to 180 TFLOP/s, 1.0 to 1.1 PFLOP/s of bf16 products (a library product in fp32 reaches 0.15).
 template <typename E, int D>
 __global__ __launch_bounds__(256, (Image<E, D>::WAVES)) void window_tile_kernel(WinArgs a, int q_tiles, uint32_t units, bool by_pair, uint32_t* fault) {
     typedef Image<E, D> I;
@@ -986,13 +991,13 @@ Plan plan_of(int64_t total_q, int n_seq, int max_q, int max_k, int hq, int hkv, 
     // Which kernel: both times estimated in microseconds.  The tile kernel walks the keys of 128 queries one tile after the
     // other; the few-query kernel spreads them over the chip but reads them once per 64 rows, with a second launch and
     // narrower matrix operands.  The constants are fitted to both kernels' times over 115 sizes a type and head size (1 to 64
-    // sequences, 5 to 200 queries, 300 to 16384 keys); by the estimate the sum of the chosen times is 1 % over the best of
-    // both, at worst a case 1.4 times.  E.g. head size 128, one sequence of 200 queries, 16 heads on 8, 16384 keys: tiles 331
-    // us, few 105; 64 sequences of them on 4096 keys: 565 and 1289.
-    static const double few_tile[2][3] = {{1.2, 1.7, 3.4}, {1.5, 2.4, 4.5}};
-    static const double one_tile[2][3] = {{0.9, 0.9, 1.17}, {1.0, 1.2, 1.5}}, all_tiles[2][3] = {{0.7, 0.8, 1.07}, {1.0, 1.7, 3.0}};
+    // sequences, 5 to 200 queries, 300 to 16384 keys); by the estimate no type's chosen times are
+    // more than 0.2 % over the best of both.  E.g. head size 128, one sequence of 200 queries, 16 heads on 8, 16384 keys: tiles
+    // 334 us, few 105; 64 sequences of them on 4096 keys: 561 and 1288.
+    static const double few_tile[2][3] = {{1.0, 1.0, 1.7}, {1.0, 2.4, 3.4}};            // of up to 32 rows; 64 rows half as much again
+    static const double one_tile[2][3] = {{0.9, 0.9, 1.0}, {0.9, 1.5, 1.8}}, all_tiles[2][3] = {{0.7, 0.7, 1.07}, {0.7, 1.3, 1.8}};
     const double wgs = (double)n_seq * hq * ((max_q + 127) / 128), waves = std::min(4, (max_q + 31) / 32 + 1);
-    const double few_us = (p.qt == 4 ? 20 : 9) + (double)base * tiles / 1024 * few_tile[wide][di];
+    const double few_us = (p.qt == 4 ? 20 : 9) + (double)base * tiles / 1024 * few_tile[wide][di] * (p.qt == 4 ? 1.5 : 1);
     const double tile_us = 9 + (double)most_tiles(max_k, std::min(max_q, 128), left, right, sinks, wide ? 32 : 64) *
                                    std::max(one_tile[wide][di], all_tiles[wide][di] * wgs * waves / 1024);
     p.few = few_us < tile_us && base < (1 << 24);
