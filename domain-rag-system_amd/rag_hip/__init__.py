@@ -1323,11 +1323,11 @@ def enc_qk_norm_rope_dev(qkv, pos, inv_freq, n_q_heads, n_kv_heads, gamma_q=None
     if kv_row is not None and kv_row.shape != (t,):
         raise ValueError("kv_row must have one entry per token")
     if q_out is None:
-        q_out = torch.empty((t, n_q_heads, d), dtype=dt, device=qkv.device)
+        q_out = qkv.new_empty((t, n_q_heads, d))
     elif q_out.shape != (t, n_q_heads, d) or (n_q_heads > 1 and q_out.stride(1) != d):
         raise ValueError("q_out must be [T, n_q_heads, D] with the heads of a row side by side")
     if k_out is None:
-        k_out = torch.empty((t, n_kv_heads, d), dtype=dt, device=qkv.device)
+        k_out = qkv.new_empty((t, n_kv_heads, d))
     rows = k_out.shape[0]
     if k_out.shape != (rows, n_kv_heads, d) or (kv_row is None and rows < t):
         raise ValueError("k_out must be [rows, n_kv_heads, D] with a row for every token")
@@ -1343,7 +1343,7 @@ def enc_qk_norm_rope_dev(qkv, pos, inv_freq, n_q_heads, n_kv_heads, gamma_q=None
                                          n_kv_heads, d, code, qp, qs if t > 1 else n_q_heads * d, kp, krs, khs, vp, vrs, vhs,
                                          _flat(kv_row, torch.int64, 'kv_row'), rows, stream), 'rag_enc_qk_norm_rope_dev')
     if v_out is None:
-        v_out = qkv.unflatten(1, (heads, d))[:, n_q_heads + n_kv_heads:]
+        v_out = qkv.as_strided((t, n_kv_heads, d), (qkv.stride(0), d, 1), qkv.storage_offset() + (n_q_heads + n_kv_heads) * d)
     return q_out, k_out, v_out
 
 
@@ -1379,7 +1379,7 @@ def enc_attention_window_dev(q, k, v, cu_q, max_q_len, k_start=None, k_len=None,
     elif k_start.shape != (n_seq,) or k_len.shape != (n_seq,):
         raise ValueError("k_start and k_len must have one entry per sequence")
     if out is None:
-        out = torch.empty((tq, hq * d), dtype=dt, device=q.device)
+        out = q.new_empty((tq, hq * d))
     elif out.shape != (tq, hq * d) or out.dtype != dt or out.stride(1) != 1:
         raise ValueError("out must be [Tq, Hq * D] of q's type with contiguous rows")
     stream = _here_and_stream(q, k, v, cu_q, k_start, k_len, out)
@@ -1447,7 +1447,7 @@ def enc_linear4_dev(x, codes, scales, offsets=None, bias=None, out=None):
     if bias is not None and bias.shape != (n,):
         raise ValueError("bias must have one entry per row of the weights")
     if out is None:
-        out = torch.empty((m, n), dtype=dt, device=x.device)
+        out = x.new_empty((m, n))
     elif out.shape != (m, n) or out.dtype != dt or out.stride(1) != 1:
         raise ValueError("out must be [M, N] of x's type with contiguous rows")
     stream = _here_and_stream(x, codes, scales, offsets, bias, out)
