@@ -124,6 +124,34 @@ __device__ void attend_row(const WinArgs& a, const Seq& sq, int j, int head, int
     }
 }
 
+// The tiles of `kt` keys that queries j0 .. j1 of a sequence see: `sinks` from the text's start, then `window` from tile w0.
+struct Tiles {
+    int sinks, w0, n;
+    __device__ int first_key(int t, int kt) const { return (t < sinks ? t : w0 + t - sinks) * kt; }
+};
+__device__ __forceinline__ Tiles tiles_of(const WinArgs& a, const Seq& sq, int j0, int j1, int kt) {
+    const Seen first = seen_by(a, sq.nk - sq.nq + j0, sq.nk), last = seen_by(a, sq.nk - sq.nq + j1, sq.nk);
+    Tiles t;
+    t.sinks = (min(a.sinks, first.lo) + kt - 1) / kt;
+    t.w0 = max(t.sinks, first.lo / kt);
+    t.n = t.sinks + max(0, (last.hi + kt - 1) / kt - t.w0);
+    return t;
+}
+
+// How the keys of a call are cut, and where the results of the spans go.
+struct FewArgs {
+    int chunks;                      // of the workgroups' rows (query * group + head of the group)
+    int spans, span;                 // workgroups along the keys, tiles of each
+    bool by_seq;                     // a partial result's row: sequence * max_q + query instead of the query's row of q
+    float2* part_ml;                 // [row][head][spans]: maximum, sum
+    float* part_o;                   // [row][head][spans][D]
+    uint64_t* done;                  // [sequence][chunk][key/value head][spans]: `token` where the span's results are written; NULL:
+    uint64_t token;                  // window_join_kernel puts them together
+};
+__device__ __forceinline__ int64_t part_at(const WinArgs& a, const FewArgs& f, const Seq& sq, int seq, int j, int head) {
+    return ((f.by_seq ? (int64_t)seq * a.max_q + j : sq.q0 + j) * a.hq + head) * f.spans;
+}
+
 // ---- a tile of 128 queries of one head per workgroup ------------------------------------------------------
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
@@ -231,14 +259,16 @@ constexpr float LAG = 8.f;           // the maximum may lag behind by this power
 // with fp32 products 602; 40 sequences of 1 to 512 tokens, 12 heads of 32, window 128: 35.5 and 58.
 // The running maximum is raised only when a score exceeds it by more than LAG (the probabilities stay below 2^LAG, in
 // the range of every type), so that the rescaling of the sums is rare.
+// SPANS: the rows are those of a key/value head (row = query * group + head of the group), the keys are cut as in FewArgs; 4
+// sequences of 64 queries, 32 heads of 128 on 8, 4000 to 16000 keys: 72 us (the few-query kernel 165, without spans 250).
 // Masked scores are -infinity; a tile that every query of the wave sees whole needs no mask, one that none sees is left
 // out.  Where keys or values hold infinities or NaN, 0 * infinity spoils rows that do not see them: every row that ends as
 // NaN is computed again by attend_row, which reads only what the row sees.
 // Bound by the matrix cores and the exponentials together: 16384 tokens, 16 heads of 128 on 8, window 4096: 0.48-0.50 ms,
 // 0.97-1.0 PFLOP/s (a library product of 8192^3 reaches 1.2); head size 64, no window: 0.36 ms for 2 x 8192, 0.77; float32:
 // 167 to 180 TFLOP/s, 1.0 to 1.1 PFLOP/s of bf16 products (a library product in fp32 reaches 0.15).
-template <typename E, int D>
-__global__ __launch_bounds__(256, (Image<E, D>::WAVES)) void window_tile_kernel(WinArgs a, int q_tiles, uint32_t units, bool by_pair, uint32_t* fault) {
+template <typename E, int D, bool SPANS>
+__global__ __launch_bounds__(256, (Image<E, D>::WAVES)) void window_tile_kernel(WinArgs a, FewArgs f, int q_tiles, uint32_t units, bool by_pair, uint32_t* fault) {
     typedef Image<E, D> I;
     typedef typename std::conditional<sizeof(E) == 4, bf16, E>::type M;          // of the matrix operands
     constexpr int KT = I::KT, KB = KT / 32, DT = D / 32, KC = I::PIECES / 2, NB = I::BUFFERS, PARTS = I::PARTS;
@@ -259,34 +289,49 @@ __global__ __launch_bounds__(256, (Image<E, D>::WAVES)) void window_tile_kernel(
     }
     if (unit >= units) return;
     const int group = a.hq / a.hkv;
-    const uint32_t u1 = unit / (uint32_t)group, u2 = u1 / (uint32_t)q_tiles;
-    const int g = (int)(unit - u1 * (uint32_t)group);
-    const int qt = q_tiles - 1 - (int)(u1 - u2 * (uint32_t)q_tiles);           // (a causal sequence's last tiles are its longest)
-    const int seq = (int)(u2 / (uint32_t)a.hkv), kvh = (int)(u2 - (uint32_t)seq * (uint32_t)a.hkv);
-    const int head = kvh * group + g;
+    const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int seq, kvh, head, span = 0, first, rows, step;         // the workgroup's rows `first` .. of `rows`: row / step is the query
+    if (SPANS) {
+        const uint32_t u1 = unit / (uint32_t)f.chunks, u2 = u1 / (uint32_t)f.spans;
+        first = (int)(unit - u1 * (uint32_t)f.chunks) * 128;
+        span = (int)(u1 - u2 * (uint32_t)f.spans);
+        seq = (int)(u2 / (uint32_t)a.hkv);
+        kvh = (int)(u2 - (uint32_t)seq * (uint32_t)a.hkv);
+        step = group;
+    } else {
+        const uint32_t u1 = unit / (uint32_t)group, u2 = u1 / (uint32_t)q_tiles;
+        first = (q_tiles - 1 - (int)(u1 - u2 * (uint32_t)q_tiles)) * 128;      // (a causal sequence's last tiles are its longest)
+        seq = (int)(u2 / (uint32_t)a.hkv);
+        kvh = (int)(u2 - (uint32_t)seq * (uint32_t)a.hkv);
+        head = kvh * group + (int)(unit - u1 * (uint32_t)group);
+        step = 1;
+    }
     Seq sq;
-    if (!load_seq(a, seq, sq, fault) || qt * 128 >= sq.nq) return;
+    if (!load_seq(a, seq, sq, fault)) return;
+    rows = sq.nq * step;
+    if (first >= rows) return;
 
-    const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int r = lane & 31, h = lane >> 5;
-    const int q0 = qt * 128 + wave * 32;                     // first query of the wave
-    const int qr = q0 + r;
-    const bool wave_on = q0 < sq.nq, row_on = qr < sq.nq;
+    const int row0 = first + wave * 32, row = row0 + r;      // of the wave, of the lane
+    const bool wave_on = row0 < rows, row_on = row < rows;
+    const int last_row = rows - 1;
+    const auto query = [&](int i) { return SPANS ? min(i, last_row) / step : min(i, last_row); };
+    const int qr = query(row);
+    if (SPANS) head = kvh * group + min(row, last_row) % step;
     const int shift = sq.nk - sq.nq;                         // position of query 0
-    const Seen mine = seen_by(a, shift + min(qr, sq.nq - 1), sq.nk);
-    const Seen w_first = seen_by(a, shift + q0, sq.nk), w_last = seen_by(a, shift + min(q0 + 31, sq.nq - 1), sq.nk);
-    const Seen t_first = seen_by(a, shift + qt * 128, sq.nk), t_last = seen_by(a, shift + min(qt * 128 + 127, sq.nq - 1), sq.nk);
+    const Seen mine = seen_by(a, shift + qr, sq.nk);
+    const Seen w_first = seen_by(a, shift + query(row0), sq.nk), w_last = seen_by(a, shift + query(row0 + 31), sq.nk);
     // the tiles of keys that some query of the workgroup sees
-    const int sink_tiles = (min(a.sinks, t_first.lo) + KT - 1) / KT;
-    const int win_tile = max(sink_tiles, t_first.lo / KT);
-    const int n_tiles = sink_tiles + max(0, (t_last.hi + KT - 1) / KT - win_tile);
+    const Tiles tiles = tiles_of(a, sq, query(first), query(first + 127), KT);
+    const int n_spans = SPANS ? max(1, (tiles.n + f.span - 1) / f.span) : 1;
+    const int t0 = SPANS ? span * f.span : 0, t1 = SPANS ? min(tiles.n, t0 + f.span) : tiles.n;
+    if (SPANS && t0 >= t1 && span > 0) return;
 
     const unsigned char* kbase = reinterpret_cast<const unsigned char*>(a.k) + (sq.k0 * a.k_row + (int64_t)kvh * a.k_head) * (int64_t)sizeof(E);
     const unsigned char* vbase = reinterpret_cast<const unsigned char*>(a.v) + (sq.k0 * a.v_row + (int64_t)kvh * a.v_head) * (int64_t)sizeof(E);
     const uint32_t k_rowb = (uint32_t)(a.k_row * (int64_t)sizeof(E)), v_rowb = (uint32_t)(a.v_row * (int64_t)sizeof(E));
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
-    auto first_key = [&](int t) { return (t < sink_tiles ? t : win_tile + t - sink_tiles) * KT; };
+    auto first_key = [&](int t) { return tiles.first_key(t, KT); };
     auto stage = [&](int t) {
         const int key0 = first_key(t);
         const int last = sq.nk - 1 - key0;                   // rows beyond the last key repeat it (masked)
@@ -338,9 +383,9 @@ __global__ __launch_bounds__(256, (Image<E, D>::WAVES)) void window_tile_kernel(
                 *reinterpret_cast<u32x4*>(dst + (value ? I::BYTES : 0) + p * I::PART + row * I::ROWB + (piece ^ (value ? I::v_swizzle(row) : I::k_swizzle(row))) * 16) = w[p];
         }
     };
-    if (n_tiles > 0) {
-        if constexpr (PARTS == 1) stage(0);
-        else fetch(0);
+    if (t0 < t1) {
+        if constexpr (PARTS == 1) stage(t0);
+        else fetch(t0);
     }
 
     // Q^T: piece 2c + h of the lane's query
@@ -348,7 +393,7 @@ __global__ __launch_bounds__(256, (Image<E, D>::WAVES)) void window_tile_kernel(
     const float scale = fabsf(a.scale);
     u32x4 qf[KC][PARTS];
     {
-        const unsigned char* qp = reinterpret_cast<const unsigned char*>(a.q) + ((sq.q0 + min(qr, sq.nq - 1)) * a.q_stride + (int64_t)head * D) * (int64_t)sizeof(E);
+        const unsigned char* qp = reinterpret_cast<const unsigned char*>(a.q) + ((sq.q0 + qr) * a.q_stride + (int64_t)head * D) * (int64_t)sizeof(E);
 #pragma unroll
         for (int c = 0; c < KC; ++c) {
             if constexpr (PARTS == 1) {
@@ -373,10 +418,10 @@ __global__ __launch_bounds__(256, (Image<E, D>::WAVES)) void window_tile_kernel(
     if constexpr (PARTS == 1) {
 #pragma unroll
         for (int t = 1; t < NB - 1; ++t)
-            if (t < n_tiles) stage(t);
-    } else if (NB == 2 && n_tiles > 0) {
-        put(0);
-        if (n_tiles > 1) fetch(1);
+            if (t0 + t < t1) stage(t0 + t);
+    } else if (NB == 2 && t0 < t1) {
+        put(t0);
+        if (t0 + 1 < t1) fetch(t0 + 1);
     }
     float m_run = NEG_BIG, l_run = 0.f;                      // l_run: the lane's own keys
     f32x16 o[DT];
@@ -385,14 +430,14 @@ __global__ __launch_bounds__(256, (Image<E, D>::WAVES)) void window_tile_kernel(
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
 
-    for (int t = 0; t < n_tiles; ++t) {
+    for (int t = t0; t < t1; ++t) {
         if constexpr (PARTS == 1) {
             // this tile's loads; those of the next NB - 2 stay in flight
-            if (NB > 2 && t + NB - 2 < n_tiles) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"((NB - 2) * (I::BYTES / 2048)) : "memory");
+            if (NB > 2 && t + NB - 2 < t1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"((NB - 2) * (I::BYTES / 2048)) : "memory");
             else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_barrier();                    // every wave has its part, and is done with the tile before
             asm volatile("" ::: "memory");
-            if (t + NB - 1 < n_tiles) stage(t + NB - 1);
+            if (t + NB - 1 < t1) stage(t + NB - 1);
         } else {
             if (NB == 1) {
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -403,8 +448,8 @@ __global__ __launch_bounds__(256, (Image<E, D>::WAVES)) void window_tile_kernel(
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_barrier();                    // the tile is there
             asm volatile("" ::: "memory");
-            if (NB == 2 && t + 1 < n_tiles) put(t + 1);
-            if (t + NB < n_tiles) fetch(t + NB);
+            if (NB == 2 && t + 1 < t1) put(t + 1);
+            if (t + NB < t1) fetch(t + NB);
         }
         const int key0 = first_key(t);
         // whether some query of the wave sees some of the tile, and whether all see all of it
@@ -507,6 +552,18 @@ __global__ __launch_bounds__(256, (Image<E, D>::WAVES)) void window_tile_kernel(
     }
     if (!wave_on) return;
 
+    if (SPANS && n_spans > 1) {
+        const float l = both_halves_sum(l_run);
+        if (!row_on) return;
+        const int64_t at = part_at(a, f, sq, seq, qr, head) + span;
+        if (h == 0) f.part_ml[at] = make_float2(m_run, l);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int gq = 0; gq < 4; ++gq)
+                *reinterpret_cast<float4*>(f.part_o + at * D + dt * 32 + 8 * gq + 4 * h) = make_float4(o[dt][4 * gq], o[dt][4 * gq + 1], o[dt][4 * gq + 2], o[dt][4 * gq + 3]);
+        return;
+    }
     const bool any_seen = mine.s + (mine.hi - mine.lo) > 0;
     const float inv = 1.f / both_halves_sum(l_run);
     bool bad = false;
@@ -546,7 +603,11 @@ __global__ __launch_bounds__(256, (Image<E, D>::WAVES)) void window_tile_kernel(
             }
         }
     }
-    for (uint32_t rest = bad_rows; rest != 0; rest &= rest - 1) attend_row<E, D>(a, sq, q0 + __builtin_ctz(rest), head, lane);
+    for (uint32_t rest = bad_rows; rest != 0; rest &= rest - 1) {
+        const int i = row0 + __builtin_ctz(rest);
+        if (SPANS) attend_row<E, D>(a, sq, i / step, kvh * group + i % step, lane);
+        else attend_row<E, D>(a, sq, i, head, lane);
+    }
 }
 
 // ---- few queries over many keys ------------------------------------------------------------------
@@ -582,20 +643,6 @@ template <> struct MmaFew<f16> {
     __device__ static f32x4 mfma(Mma<f16>::x8 a, Mma<f16>::x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 
-// The tiles of `kt` keys that queries j0 .. j1 of a sequence see: `sinks` from the text's start, then `window` from tile w0.
-struct Tiles {
-    int sinks, w0, n;
-    __device__ int first_key(int t, int kt) const { return (t < sinks ? t : w0 + t - sinks) * kt; }
-};
-__device__ __forceinline__ Tiles tiles_of(const WinArgs& a, const Seq& sq, int j0, int j1, int kt) {
-    const Seen first = seen_by(a, sq.nk - sq.nq + j0, sq.nk), last = seen_by(a, sq.nk - sq.nq + j1, sq.nk);
-    Tiles t;
-    t.sinks = (min(a.sinks, first.lo) + kt - 1) / kt;
-    t.w0 = max(t.sinks, first.lo / kt);
-    t.n = t.sinks + max(0, (last.hi + kt - 1) / kt - t.w0);
-    return t;
-}
-
 __device__ __forceinline__ float quarters_max(float v) {     // over the four lanes that share lane % 16
     const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     v = fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
@@ -607,19 +654,6 @@ __device__ __forceinline__ float quarters_sum(float v) {
     v = __uint_as_float(p[0]) + __uint_as_float(p[1]);
     const auto q = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(q[0]) + __uint_as_float(q[1]);
-}
-
-struct FewArgs {
-    int chunks;                      // of 16 * QT rows
-    int spans, span;                 // workgroups along the keys, tiles of each
-    bool by_seq;                     // a partial result's row: sequence * max_q + query instead of the query's row of q
-    float2* part_ml;                 // [row][head][spans]: maximum, sum
-    float* part_o;                   // [row][head][spans][D]
-    uint64_t* done;                  // [sequence][chunk][key/value head][spans]: `token` where the span's results are written; NULL:
-    uint64_t token;                  // window_join_kernel puts them together
-};
-__device__ __forceinline__ int64_t part_at(const WinArgs& a, const FewArgs& f, const Seq& sq, int seq, int j, int head) {
-    return ((f.by_seq ? (int64_t)seq * a.max_q + j : sq.q0 + j) * a.hq + head) * f.spans;
 }
 
 // Values that workgroups on other XCDs read or wrote in the same launch: past the L2, which is an XCD's own.
@@ -946,7 +980,7 @@ __global__ __launch_bounds__(64 * (FewImage<E, D>::NW)) void window_few_kernel(W
 
 // The results of one query row and head whose chunks of rows are not put together by window_few_kernel, a wave each.
 template <typename E, int D>
-__global__ __launch_bounds__(256) void window_join_kernel(WinArgs a, FewArgs f, int rows_of_chunk) {
+__global__ __launch_bounds__(256) void window_join_kernel(WinArgs a, FewArgs f, int rows_of_chunk, int kt) {
     const int group = a.hq / a.hkv, lane = threadIdx.x & 63;
     const int per_seq = (a.max_q * a.hq + 3) / 4;
     const int seq = (int)(blockIdx.x / per_seq);
@@ -956,15 +990,16 @@ __global__ __launch_bounds__(256) void window_join_kernel(WinArgs a, FewArgs f, 
     if (!load_seq(a, seq, sq, nullptr) || j >= sq.nq) return;
     const int chunk = (j * group + head % group) / rows_of_chunk;
     const int last = min((chunk + 1) * rows_of_chunk, sq.nq * group) - 1;
-    const Tiles tiles = tiles_of(a, sq, chunk * rows_of_chunk / group, last / group, FewImage<E, D>::KT);
+    const Tiles tiles = tiles_of(a, sq, chunk * rows_of_chunk / group, last / group, kt);
     const int n = (tiles.n + f.span - 1) / f.span;
     if (n > 1) join_row<E, D, false>(a, f, sq, seq, j, head, n, lane);          // (one span's results are stored as they are)
 }
 
 // How a call runs, from its sizes alone (the workspace is computed from the same).
+enum Kernel { TILE, FEW, TILE_SPANS };
 struct Plan {
-    bool few;
-    int qt, chunks, spans, span;     // few: 16-row columns of a workgroup, its row chunks, spans along the keys
+    Kernel kernel;
+    int qt, chunks, spans, span;     // 16-row columns of a workgroup (few), chunks of the rows, spans along the keys
     int64_t parts;                   // query rows * heads * spans whose partial results the workspace holds
     int64_t marks;                   // 0: window_join_kernel puts them together
     int64_t bytes(int D) const { return marks * 8 + parts * (D + 2) * 4; }
@@ -978,30 +1013,45 @@ int64_t most_tiles(int max_k, int queries, int left, int right, int sinks, int k
 }
 
 Plan plan_of(int64_t total_q, int n_seq, int max_q, int max_k, int hq, int hkv, int D, int left, int right, int sinks, int size) {
-    Plan p{};
     const int group = hq / hkv, wide = size == 4, di = D == 32 ? 0 : D == 64 ? 1 : 2;
-    const int64_t rows = (int64_t)max_q * group;
-    if (rows > 4096) return p;                               // (never the faster there, and the numbers below stay small)
-    p.qt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-    p.chunks = (int)((rows + 16 * p.qt - 1) / (16 * p.qt));
-    const int kt = wide ? 16 : 32;
-    const int64_t tiles = most_tiles(max_k, max_q, left, right, sinks, kt);
-    const int64_t base = (int64_t)n_seq * hkv * p.chunks;
+    const int64_t rows = (int64_t)max_q * group, pairs = (int64_t)n_seq * hkv;
 
-    // Which kernel: both times estimated in microseconds.  The tile kernel walks the keys of 128 queries one tile after the
-    // other; the few-query kernel spreads them over the chip but reads them once per 64 rows, with a second launch and
-    // narrower matrix operands.  The constants are fitted to both kernels' times over 115 sizes a type and head size (1 to 64
-    // sequences, 5 to 200 queries, 300 to 16384 keys); by the estimate no type's chosen times are
-    // more than 0.2 % over the best of both.  E.g. head size 128, one sequence of 200 queries, 16 heads on 8, 16384 keys: tiles
-    // 334 us, few 105; 64 sequences of them on 4096 keys: 561 and 1288.
-    static const double few_tile[2][3] = {{1.0, 1.0, 1.7}, {1.0, 2.4, 3.4}};            // of up to 32 rows; 64 rows half as much again
+    // Which kernel: the times estimated in microseconds.  The tile kernel walks the keys of 128 queries one tile after the
+    // other; with spans it takes the rows of a key/value head together and spreads them and their keys over the chip, with a second
+    // launch; the few-query kernel spreads them too but reads them once per 64 rows, with narrower matrix operands.  The
+    // constants are fitted to the kernels' times over 197 sizes a type and head size (1 to 32 sequences, 9 to 1500 queries, 600 to
+    // 16384 keys); the chosen times are 1 % over the best of the three on average, without the spans 30 %.  E.g. head size 128,
+    // bf16, 16 heads on 8, 4 sequences of 200 queries on 4096 keys: few 102 us, spans 58, tiles 91; of 9 queries: 21, 26, 85.
+    static const double few_tile[2][3] = {{1.0, 1.0, 1.7}, {1.0, 2.4, 3.4}};            // of 17 to 32 rows
     static const double one_tile[2][3] = {{0.9, 0.9, 1.0}, {0.9, 1.5, 1.8}}, all_tiles[2][3] = {{0.7, 0.7, 1.07}, {0.7, 1.3, 1.8}};
-    const double wgs = (double)n_seq * hq * ((max_q + 127) / 128), waves = std::min(4, (max_q + 31) / 32 + 1);
-    const double few_us = (p.qt == 4 ? 20 : 9) + (double)base * tiles / 1024 * few_tile[wide][di] * (p.qt == 4 ? 1.5 : 1);
-    const double tile_us = 9 + (double)most_tiles(max_k, std::min(max_q, 128), left, right, sinks, wide ? 32 : 64) *
-                                   std::max(one_tile[wide][di], all_tiles[wide][di] * wgs * waves / 1024);
-    p.few = few_us < tile_us && base < (1 << 24);
-    if (!p.few) return p;
+    static const int on_cu[2][3] = {{4, 3, 2}, {4, 2, 1}};   // workgroups of the tile kernel
+    const auto tile_time = [&](int64_t tiles, double wgs, int64_t rows_of_wg) {
+        return (double)tiles * std::max(one_tile[wide][di], all_tiles[wide][di] * wgs * std::min<int64_t>(4, (rows_of_wg + 31) / 32 + 1) / 1024);
+    };
+    Plan tile{}, few{}, cut{};
+    const int kt_tile = wide ? 32 : 64;
+    const double tile_us = 9 + tile_time(most_tiles(max_k, std::min(max_q, 128), left, right, sinks, kt_tile), (double)n_seq * hq * ((max_q + 127) / 128), max_q);
+
+    few.kernel = FEW;
+    few.qt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    few.chunks = (int)std::min<int64_t>(1 << 24, (rows + 16 * few.qt - 1) / (16 * few.qt));
+    const int kt = wide ? 16 : 32;
+    const int64_t tiles = most_tiles(max_k, max_q, left, right, sinks, kt), base = std::min<int64_t>(1 << 24, pairs * few.chunks);
+    const double few_us = (few.qt == 4 ? 18 : 9) + (double)base * tiles / 1024 * few_tile[wide][di] * (few.qt == 4 ? 2.1 : few.qt == 1 && wide ? 0.5 : 1);
+
+    cut.kernel = TILE_SPANS;
+    cut.chunks = (int)std::min<int64_t>(1 << 24, (rows + 127) / 128);
+    const int64_t cut_tiles = most_tiles(max_k, (int)std::min<int64_t>(max_q, 127 / group + 2), left, right, sinks, kt_tile);
+    const int64_t cut_base = std::min<int64_t>(1 << 24, pairs * cut.chunks), cut_cuts = std::max<int64_t>(1, 256 * on_cu[wide][di] / cut_base);
+    cut.span = (int)std::max<int64_t>(8, (cut_tiles + cut_cuts - 1) / cut_cuts);
+    cut.spans = (int)((cut_tiles + cut.span - 1) / cut.span);
+    cut.parts = cut.spans > 1 ? std::min(total_q, (int64_t)n_seq * max_q) * hq * cut.spans : 0;
+    double cut_us = (cut.spans > 1 ? 15 : 9) + tile_time(std::min<int64_t>(cut.span, cut_tiles), (double)cut_base * cut.spans, rows) +
+                    (double)cut.parts * (D + 2) / 1e6;       // (8 bytes each, written and read)
+    if (rows <= 16) cut_us = tile_us;                        // columns of the matrix products mostly empty (16 sequences of unlike lengths, one
+                                                             // token: 227 us, few 188)
+    if (few_us >= std::min(tile_us, cut_us) || base == 1 << 24) return cut_us < 0.9 * tile_us && cut_base < 1 << 24 ? cut : tile;
+    Plan& p = few;
 
     // A workgroup's start, the filling of its buffers and its end cost as much as some 8 tiles a wave, so the workgroups that are on
     // the chip at once (256 compute units by what their LDS leaves room for) run one round: one token over 32768 keys of 8 heads
@@ -1024,49 +1074,67 @@ Plan plan_of(int64_t total_q, int n_seq, int max_q, int max_k, int hq, int hkv, 
     return p;
 }
 
-template <typename T, int D, int QT>
-int window_few(const WinArgs& a, const Plan& p, void* work, hipStream_t stream) {
+FewArgs few_args(const WinArgs& a, const Plan& p, int D, void* work) {
+    static std::atomic<uint64_t> tokens{(uint64_t)std::chrono::steady_clock::now().time_since_epoch().count() * 0x9e3779b97f4a7c15ull | 1};
     FewArgs f;
     f.chunks = p.chunks; f.spans = p.spans; f.span = p.span;
     f.by_seq = (int64_t)a.n_seq * a.max_q < a.total_q;       // rows of no sequence take no room
-    static std::atomic<uint64_t> tokens{(uint64_t)std::chrono::steady_clock::now().time_since_epoch().count() * 0x9e3779b97f4a7c15ull | 1};
     f.done = p.marks > 0 ? reinterpret_cast<uint64_t*>(work) : nullptr;
     f.token = p.marks > 0 ? tokens.fetch_add(2) : 0;         // (odd: never what a call leaves)
     f.part_o = reinterpret_cast<float*>(reinterpret_cast<uint64_t*>(work) + p.marks);
     f.part_ml = reinterpret_cast<float2*>(f.part_o + p.parts * D);
+    return f;
+}
+
+template <typename T, int D>
+int window_join(const WinArgs& a, const FewArgs& f, int rows_of_chunk, int kt, hipStream_t stream) {
+    const int64_t joins = (int64_t)a.n_seq * (((int64_t)a.max_q * a.hq + 3) / 4);
+    RAG_REQUIRE(joins < (1ll << 31), RAG_ELIMIT, "rag_enc_attention_window: too many query rows");
+    window_join_kernel<T, D><<<(unsigned)joins, 256, 0, stream>>>(a, f, rows_of_chunk, kt);
+    RAG_HIP_TRY(hipGetLastError());
+    return RAG_OK;
+}
+
+template <typename T, int D, int QT>
+int window_few(const WinArgs& a, const Plan& p, void* work, hipStream_t stream) {
+    const FewArgs f = few_args(a, p, D, work);
     const int64_t grid = (int64_t)a.n_seq * p.spans * p.chunks * a.hkv;
     RAG_REQUIRE(grid < (1ll << 31), RAG_ELIMIT, "rag_enc_attention_window: too many sequences");
     constexpr size_t lds = FewImage<T, D>::lds(16 * QT);
     RAG_GRANT_LDS((window_few_kernel<T, D, QT>), lds);
     window_few_kernel<T, D, QT><<<(unsigned)grid, 64 * FewImage<T, D>::NW, lds, stream>>>(a, f, rag_fault_word());
     RAG_HIP_TRY(hipGetLastError());
-    if (p.spans > 1 && p.marks == 0) {
-        const int64_t joins = (int64_t)a.n_seq * (((int64_t)a.max_q * a.hq + 3) / 4);
-        RAG_REQUIRE(joins < (1ll << 31), RAG_ELIMIT, "rag_enc_attention_window: too many query rows");
-        window_join_kernel<T, D><<<(unsigned)joins, 256, 0, stream>>>(a, f, 16 * QT);
-        RAG_HIP_TRY(hipGetLastError());
-    }
-    return RAG_OK;
+    return p.spans > 1 && p.marks == 0 ? window_join<T, D>(a, f, 16 * QT, FewImage<T, D>::KT, stream) : RAG_OK;
 }
 
 template <typename T, int D>
 int window_launch(const WinArgs& a, void* work, int64_t work_bytes, hipStream_t stream) {
     const Plan p = plan_of(a.total_q, a.n_seq, a.max_q, a.max_k, a.hq, a.hkv, D, a.left, a.right, a.sinks, (int)sizeof(T));
-    if (p.few) {
-        RAG_REQUIRE(p.bytes(D) <= work_bytes, RAG_EINVAL, "rag_enc_attention_window: the workspace holds %lld bytes, %lld are needed",
-                    (long long)work_bytes, (long long)p.bytes(D));
+    RAG_REQUIRE(p.bytes(D) <= work_bytes, RAG_EINVAL, "rag_enc_attention_window: the workspace holds %lld bytes, %lld are needed",
+                (long long)work_bytes, (long long)p.bytes(D));
+    if (p.kernel == FEW) {
         if (p.qt == 1) return window_few<T, D, 1>(a, p, work, stream);
         if (p.qt == 2) return window_few<T, D, 2>(a, p, work, stream);
         return window_few<T, D, 4>(a, p, work, stream);
     }
+    constexpr size_t lds = 2 * (size_t)Image<T, D>::BUFFERS * Image<T, D>::BYTES;
+    const int64_t pairs = (int64_t)a.n_seq * a.hkv;
+    if (p.kernel == TILE_SPANS) {
+        const FewArgs f = few_args(a, p, D, work);
+        const int64_t units = pairs * p.chunks * p.spans, grid = (units + 7) / 8 * 8;
+        RAG_REQUIRE(grid < (1ll << 31), RAG_ELIMIT, "rag_enc_attention_window: too many query tiles");
+        RAG_GRANT_LDS((window_tile_kernel<T, D, true>), lds);
+        window_tile_kernel<T, D, true><<<(unsigned)grid, 256, lds, stream>>>(a, f, 0, (uint32_t)units, false, rag_fault_word());
+        RAG_HIP_TRY(hipGetLastError());
+        return p.spans > 1 ? window_join<T, D>(a, f, 128, Image<T, D>::KT, stream) : RAG_OK;
+    }
     const int q_tiles = (a.max_q + 127) / 128;
-    const int64_t pairs = (int64_t)a.n_seq * a.hkv, units = pairs * q_tiles * (a.hq / a.hkv);
+    const int64_t units = pairs * q_tiles * (a.hq / a.hkv);
     const bool by_pair = pairs % 8 == 0 || pairs >= 64;
     const int64_t grid = by_pair ? (pairs + 7) / 8 * 8 * q_tiles * (a.hq / a.hkv) : (units + 7) / 8 * 8;
     RAG_REQUIRE(grid < (1ll << 31), RAG_ELIMIT, "rag_enc_attention_window: too many query tiles");
-    constexpr size_t lds = 2 * (size_t)Image<T, D>::BUFFERS * Image<T, D>::BYTES;
-    RAG_GRANT_LDS((window_tile_kernel<T, D>), lds);
-    window_tile_kernel<T, D><<<(unsigned)grid, 256, lds, stream>>>(a, q_tiles, (uint32_t)units, by_pair, rag_fault_word());
+    RAG_GRANT_LDS((window_tile_kernel<T, D, false>), lds);
+    window_tile_kernel<T, D, false><<<(unsigned)grid, 256, lds, stream>>>(a, FewArgs{}, q_tiles, (uint32_t)units, by_pair, rag_fault_word());
     RAG_HIP_TRY(hipGetLastError());
     return RAG_OK;
 }

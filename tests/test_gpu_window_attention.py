@@ -492,3 +492,55 @@ def test_two_streams_at_once():
                 got[i].append(call(i))
     torch.cuda.synchronize()
     assert all(torch.equal(x, want[i]) for i in range(2) for x in got[i])
+
+
+@pytest.mark.parametrize('kind', list(TYPES))
+@pytest.mark.parametrize('hq,hkv,d', [(6, 2, 64), (8, 1, 32), (4, 4, 128), (12, 1, 128)])
+@pytest.mark.parametrize('left,right,sinks', [(-1, -1, 0), (-1, 0, 0), (900, 0, 5), (300, 200, 1)])
+def test_pieces_of_a_text_behind_kept_keys(kind, hq, hkv, d, left, right, sinks):
+    # some tens or hundreds of queries on long keys: the rows of a key/value head in tiles, the keys in spans
+    import rag_hip
+    dt, dev = TYPES[kind], _dev()
+    q_lens, lens = [1, 0, 37, 210, 70], [3000, 10, 37, 2100, 40]
+    g = _gen(hq * 7 + d)
+    q = torch.randn((sum(q_lens) + 3, hq, d), generator=g, device=dev).to(dt)
+    k, v = (torch.randn((sum(lens), hkv, d), generator=g, device=dev).to(dt) for _ in range(2))
+    k0 = [sum(lens[:i]) for i in range(len(lens))]
+    out = torch.full((q.shape[0], hq * d), 5.0, dtype=dt, device=dev)
+    kw = dict(k_start=torch.tensor(k0, dtype=torch.int64, device=dev), k_len=torch.tensor(lens, dtype=torch.int32, device=dev), max_k_len=3000,
+              window_left=left, window_right=right, n_sinks=sinks)
+    rag_hip.enc_attention_window_dev(q, k, v, _cu(q_lens), 210, out=out, **kw)
+    assert bool((out[sum(q_lens):] == 5.0).all())
+    _check(out, q, k, v, q_lens, list(zip(k0, lens)), left, right, sinks, d ** -0.5)
+    if right == 0:
+        # keys and values behind the first 150 queries of the fourth sequence hold what must not reach them, key by key
+        # (rows that meet them are computed again in another order: as near the formula, but not the same bits)
+        kn, vn = k.clone(), v.clone()
+        hidden = k0[3] + 2100 - 60
+        kn[hidden::2], vn[hidden::3] = math.nan, math.inf
+        again = rag_hip.enc_attention_window_dev(q, kn, vn, _cu(q_lens), 210, **kw)
+        _check(again[38:188], q[38:188], k, v, [150], [(k0[3], 2100 - 60)], left, right, sinks, d ** -0.5)
+
+
+def test_pieces_of_a_text_in_a_captured_graph():
+    import rag_hip
+    dt, dev, hq, hkv, d, nq, nk = torch.bfloat16, _dev(), 8, 2, 64, 90, 7000
+    g = _gen(5)
+    q = torch.randn((nq, hq, d), generator=g, device=dev).to(dt)
+    k, v = (torch.randn((nk, hkv, d), generator=g, device=dev).to(dt) for _ in range(2))
+    cu, k_start, k_len = _cu([nq]), torch.zeros(1, dtype=torch.int64, device=dev), torch.full((1,), nk, dtype=torch.int32, device=dev)
+
+    def call():
+        return rag_hip.enc_attention_window_dev(q, k, v, cu, nq, k_start=k_start, k_len=k_len, max_k_len=nk, window_right=0)
+    graph = torch.cuda.CUDAGraph()
+    call()
+    with torch.cuda.graph(graph):
+        out = call()
+    for n in (7000, 300, 90, 7000, 2501):
+        k_len.fill_(n)
+        q.mul_(0.95)
+        graph.replay()
+        want = call()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), n
+        _check(want, q, k, v, [nq], [(0, n)], -1, 0, 0, d ** -0.5)
