@@ -1401,7 +1401,9 @@ def enc_attention_window_dev(q, k, v, cu_q, max_q_len, k_start=None, k_len=None,
 
 @functools.lru_cache(maxsize=4096)
 def _window_workspace(*sizes):
-    """rag_enc_attention_window_workspace, which goes by the sizes alone."""
+    """rag_enc_attention_window_workspace, which goes by the sizes alone; they must fit the C interface's 32 bits."""
+    if max(sizes[1:]) > 0x7fffffff or min(sizes[1:]) < -0x80000000:
+        raise ValueError(f"lengths, windows and sinks must be below 2^31 (a window of -1 has no limit): {sizes}")
     return load_library().rag_enc_attention_window_workspace(*sizes)
 
 
@@ -1440,6 +1442,8 @@ def enc_linear4_dev(x, codes, scales, offsets=None, bias=None, out=None):
     if x.dim() != 2 or codes.dim() != 2 or scales.dim() != 2 or not x.is_cuda or x.stride(1) != 1:
         raise ValueError("x must be a 2-d GPU tensor with contiguous rows, codes and scales 2-d")
     (m, k), (n, half), (sn, groups) = x.shape, codes.shape, scales.shape
+    if n > 0x7fffffff or k > 0x7fffffff:
+        raise ValueError("the weights must have less than 2^31 rows and columns")
     if half * 2 != k or sn != n or groups < 1 or k % groups:
         raise ValueError("codes must be [N, K / 2] and scales [N, K / group]")
     if offsets is not None and offsets.shape != scales.shape:

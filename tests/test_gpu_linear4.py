@@ -141,3 +141,10 @@ def test_another_stream_and_a_replayed_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y2, rag_hip.enc_linear4_dev(x, codes, scales, off, bias)), i
+
+
+def test_weights_beyond_the_interface_are_refused():
+    import rag_hip
+    x = torch.zeros((1, 32), device='cuda')
+    with pytest.raises(ValueError, match='2\\^31'):
+        rag_hip.enc_linear4_dev(x, torch.zeros((1, 16), dtype=torch.uint8, device='cuda').expand(1 << 32, 16), torch.zeros((1, 1), device='cuda').expand(1 << 32, 1))

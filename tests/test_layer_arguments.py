@@ -126,3 +126,14 @@ def test_rope_inv_freq():
     import rag_hip
     f = rag_hip.rope_inv_freq(8, 10000.0, device='cpu')
     assert f.dtype == torch.float64 and np.allclose(f.numpy(), [1, 0.1, 0.01, 0.001], rtol=1e-15)
+
+
+@pytest.mark.parametrize('at', range(1, 10))
+def test_sizes_beyond_the_interface_are_refused(at):
+    # ctypes would pass 2^32 as 0: a window of one key instead of one beyond every length
+    import rag_hip
+    sizes = [4, 1, 4, 4, 2, 2, 64, -1, 0, 0, 1]
+    assert rag_hip._window_workspace(*sizes) == 0
+    sizes[at] = 1 << 32
+    with pytest.raises(ValueError, match='2\\^31'):
+        rag_hip._window_workspace(*sizes)
