@@ -195,7 +195,7 @@ extern "C" int rag_enc_qk_norm_rope_dev(const void* d_qkv, int64_t qkv_stride, c
     a.chunks = (a.heads + per_wave - 1) / per_wave;
     RAG_REQUIRE(n_tokens < (1ll << 40), RAG_ELIMIT, "%s: too many tokens", me);
     const int64_t grid = ceil_div64(n_tokens * a.chunks, ROPE_NT / 64);
-    RAG_REQUIRE(grid < (1ll << 31), RAG_ELIMIT, "%s: too many tokens", me);
+    RAG_REQUIRE(grid < (1ll << 24), RAG_ELIMIT, "%s: too many tokens", me);
     hipStream_t stream = (hipStream_t)stream_;
     if (dtype == RAG_DTYPE_F32) return rope_by_dim<float>(a, head_dim, interleaved != 0, (unsigned)grid, stream);
     if (dtype == RAG_DTYPE_BF16) return rope_by_dim<bf16>(a, head_dim, interleaved != 0, (unsigned)grid, stream);

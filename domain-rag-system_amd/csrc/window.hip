@@ -1089,7 +1089,7 @@ FewArgs few_args(const WinArgs& a, const Plan& p, int D, void* work) {
 template <typename T, int D>
 int window_join(const WinArgs& a, const FewArgs& f, int rows_of_chunk, int kt, hipStream_t stream) {
     const int64_t joins = (int64_t)a.n_seq * (((int64_t)a.max_q * a.hq + 3) / 4);
-    RAG_REQUIRE(joins < (1ll << 31), RAG_ELIMIT, "rag_enc_attention_window: too many query rows");
+    RAG_REQUIRE(joins < (1ll << 24), RAG_ELIMIT, "rag_enc_attention_window: too many query rows");
     window_join_kernel<T, D><<<(unsigned)joins, 256, 0, stream>>>(a, f, rows_of_chunk, kt);
     RAG_HIP_TRY(hipGetLastError());
     return RAG_OK;
@@ -1099,7 +1099,7 @@ template <typename T, int D, int QT>
 int window_few(const WinArgs& a, const Plan& p, void* work, hipStream_t stream) {
     const FewArgs f = few_args(a, p, D, work);
     const int64_t grid = (int64_t)a.n_seq * p.spans * p.chunks * a.hkv;
-    RAG_REQUIRE(grid < (1ll << 31), RAG_ELIMIT, "rag_enc_attention_window: too many sequences");
+    RAG_REQUIRE(grid < (1ll << 24), RAG_ELIMIT, "rag_enc_attention_window: too many sequences");
     constexpr size_t lds = FewImage<T, D>::lds(16 * QT);
     RAG_GRANT_LDS((window_few_kernel<T, D, QT>), lds);
     window_few_kernel<T, D, QT><<<(unsigned)grid, 64 * FewImage<T, D>::NW, lds, stream>>>(a, f, rag_fault_word());
@@ -1122,7 +1122,7 @@ int window_launch(const WinArgs& a, void* work, int64_t work_bytes, hipStream_t 
     if (p.kernel == TILE_SPANS) {
         const FewArgs f = few_args(a, p, D, work);
         const int64_t units = pairs * p.chunks * p.spans, grid = (units + 7) / 8 * 8;
-        RAG_REQUIRE(grid < (1ll << 31), RAG_ELIMIT, "rag_enc_attention_window: too many query tiles");
+        RAG_REQUIRE(grid < (1ll << 24), RAG_ELIMIT, "rag_enc_attention_window: too many query tiles");
         RAG_GRANT_LDS((window_tile_kernel<T, D, true>), lds);
         window_tile_kernel<T, D, true><<<(unsigned)grid, 256, lds, stream>>>(a, f, 0, (uint32_t)units, false, rag_fault_word());
         RAG_HIP_TRY(hipGetLastError());
@@ -1132,7 +1132,7 @@ int window_launch(const WinArgs& a, void* work, int64_t work_bytes, hipStream_t 
     const int64_t units = pairs * q_tiles * (a.hq / a.hkv);
     const bool by_pair = pairs % 8 == 0 || pairs >= 64;
     const int64_t grid = by_pair ? (pairs + 7) / 8 * 8 * q_tiles * (a.hq / a.hkv) : (units + 7) / 8 * 8;
-    RAG_REQUIRE(grid < (1ll << 31), RAG_ELIMIT, "rag_enc_attention_window: too many query tiles");
+    RAG_REQUIRE(grid < (1ll << 24), RAG_ELIMIT, "rag_enc_attention_window: too many query tiles");
     RAG_GRANT_LDS((window_tile_kernel<T, D, false>), lds);
     window_tile_kernel<T, D, false><<<(unsigned)grid, 256, lds, stream>>>(a, FewArgs{}, q_tiles, (uint32_t)units, by_pair, rag_fault_word());
     RAG_HIP_TRY(hipGetLastError());

@@ -137,3 +137,9 @@ def test_sizes_beyond_the_interface_are_refused(at):
     sizes[at] = 1 << 32
     with pytest.raises(ValueError, match='2\\^31'):
         rag_hip._window_workspace(*sizes)
+
+
+def test_calls_of_more_workgroups_than_a_launch_takes_are_refused():
+    n = 1 << 28                                               # 2^26 workgroups of 256 threads
+    assert _rope(t=n, rows=n)[0] == -5
+    assert _window(tq=n, tk=n, n=n)[0] == -5
