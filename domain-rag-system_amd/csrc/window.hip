@@ -1014,7 +1014,7 @@ int64_t most_tiles(int max_k, int queries, int left, int right, int sinks, int k
 
 Plan plan_of(int64_t total_q, int n_seq, int max_q, int max_k, int hq, int hkv, int D, int left, int right, int sinks, int size) {
     const int group = hq / hkv, wide = size == 4, di = D == 32 ? 0 : D == 64 ? 1 : 2;
-    const int64_t rows = (int64_t)max_q * group, pairs = (int64_t)n_seq * hkv;
+    const int64_t rows = (int64_t)max_q * group, pairs = std::min<int64_t>(1 << 24, (int64_t)n_seq * hkv);      // (caps: no overflow below)
 
     // Which kernel: the times estimated in microseconds.  The tile kernel walks the keys of 128 queries one tile after the
     // other; with spans it takes the rows of a key/value head together and spreads them and their keys over the chip, with a second

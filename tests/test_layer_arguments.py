@@ -143,3 +143,15 @@ def test_calls_of_more_workgroups_than_a_launch_takes_are_refused():
     n = 1 << 28                                               # 2^26 workgroups of 256 threads
     assert _rope(t=n, rows=n)[0] == -5
     assert _window(tq=n, tk=n, n=n)[0] == -5
+
+
+def test_workspace_of_many_sequences_and_heads_does_not_overflow():
+    import rag_hip
+    f = rag_hip.load_library().rag_enc_attention_window_workspace
+    big, most = (1 << 31) - 1, (1 << 30) - 1
+    for hq, hkv in ((4096, 4096), (4096, 2048), (4096, 1), (1, 1)):
+        for max_q in (1, 5, 100, 1 << 20, most):
+            for max_k in (0, 1, 70000, most):
+                for dtype in (0, 1):
+                    for window in ((-1, -1, 0), (0, 0, 0), (big, big, big)):
+                        assert f(big, big, max_q, max_k, hq, hkv, 128, *window, dtype) == 0       # they fill the chip: nothing is cut
