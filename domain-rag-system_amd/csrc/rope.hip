@@ -13,7 +13,7 @@
 // a turn in 64 bits (a 32-bit product is off by 2^-24 of the angle itself, 0.002 radians at position 32768) and only
 // the sine and cosine of the remainder are taken in 32 bits, so there is no table to read or to size.
 // Measured: 16384 tokens of 32 query and 8 key heads of 128, bf16, 70.6 us, 4.75 TB/s (a large copy moves 4.7); 65536 tokens
-// of 16 and 8 heads of 128, half of each rotated, f16, 161 us, 5.0 TB/s; one token 4.2 us, the launch.
+// of 16 and 8 heads of 128, half of each rotated, f16, 161 us, 5.0 TB/s; one token 2.8 us, of which an empty launch is 1.6.
 #include "common.h"
 
 namespace {
@@ -41,9 +41,9 @@ struct RopeArgs {
 };
 
 constexpr int ROPE_NT = 256;
-constexpr int ROPE_U = 4;             // heads a lane takes, all their loads issued before the first is used
 
-template <typename T, int D, bool INTER>
+// U: heads a lane takes, all their loads issued before the first is used
+template <typename T, int D, bool INTER, int U>
 __global__ __launch_bounds__(ROPE_NT) void qk_norm_rope_kernel(RopeArgs a, uint32_t* fault) {
     typedef typename Vec4<T>::type v4;
     constexpr int L = D / 8;          // lanes of a head
@@ -59,10 +59,10 @@ __global__ __launch_bounds__(ROPE_NT) void qk_norm_rope_kernel(RopeArgs a, uint3
     const int off_b = INTER || !turns ? 8 * p + 4 : 4 * p + a.rot / 2;
 
     const T* row = reinterpret_cast<const T*>(a.qkv) + t * a.stride;
-    v4 xa[ROPE_U], xb[ROPE_U];
+    v4 xa[U], xb[U];
 #pragma unroll
-    for (int u = 0; u < ROPE_U; ++u) {
-        const int head = (chunk * ROPE_U + u) * HPW + lane / L;
+    for (int u = 0; u < U; ++u) {
+        const int head = (chunk * U + u) * HPW + lane / L;
         if (head < a.heads) {
             xa[u] = *reinterpret_cast<const v4*>(row + (int64_t)head * D + off_a);
             xb[u] = *reinterpret_cast<const v4*>(row + (int64_t)head * D + off_b);
@@ -84,8 +84,8 @@ __global__ __launch_bounds__(ROPE_NT) void qk_norm_rope_kernel(RopeArgs a, uint3
         }
     }
 #pragma unroll
-    for (int u = 0; u < ROPE_U; ++u) {
-        const int head = (chunk * ROPE_U + u) * HPW + lane / L;
+    for (int u = 0; u < U; ++u) {
+        const int head = (chunk * U + u) * HPW + lane / L;
         if (head >= a.heads) continue;                       // (the lanes of a head stay together)
         const bool is_q = head < a.hq, is_v = head >= a.hq + a.hkv;
         T* dst;
@@ -141,19 +141,32 @@ __global__ __launch_bounds__(ROPE_NT) void qk_norm_rope_kernel(RopeArgs a, uint3
     }
 }
 
-template <typename T, int D>
-int rope_launch(const RopeArgs& a, bool inter, unsigned grid, hipStream_t stream) {
-    if (inter) qk_norm_rope_kernel<T, D, true><<<grid, ROPE_NT, 0, stream>>>(a, rag_fault_word());
-    else qk_norm_rope_kernel<T, D, false><<<grid, ROPE_NT, 0, stream>>>(a, rag_fault_word());
+template <typename T, int D, int U>
+int rope_launch(RopeArgs a, bool inter, hipStream_t stream) {
+    const int per_wave = 64 / (D / 8) * U;
+    a.chunks = (a.heads + per_wave - 1) / per_wave;
+    const int64_t grid = ceil_div64(a.n_tokens * a.chunks, ROPE_NT / 64);
+    RAG_REQUIRE(grid < (1ll << 24), RAG_ELIMIT, "rag_enc_qk_norm_rope: too many tokens");
+    if (inter) qk_norm_rope_kernel<T, D, true, U><<<(unsigned)grid, ROPE_NT, 0, stream>>>(a, rag_fault_word());
+    else qk_norm_rope_kernel<T, D, false, U><<<(unsigned)grid, ROPE_NT, 0, stream>>>(a, rag_fault_word());
     RAG_HIP_TRY(hipGetLastError());
     return RAG_OK;
 }
 
+// One head a lane while that leaves the chip no more than 16 waves a compute unit: less to do one after the other (16 + 8
+// heads of 128, bf16: one token 2.8 us, with four heads 4.3, 512 tokens 4.0 and 5.2).  Beyond that four: more bytes in
+// flight and the angles for four heads at once (8192 tokens 23.7 us, with one head 30.5).
+template <typename T, int D>
+int rope_by_size(const RopeArgs& a, bool inter, hipStream_t stream) {
+    const int64_t waves = a.n_tokens * ((a.heads + 512 / D - 1) / (512 / D));
+    return waves <= 4096 ? rope_launch<T, D, 1>(a, inter, stream) : rope_launch<T, D, 4>(a, inter, stream);
+}
+
 template <typename T>
-int rope_by_dim(const RopeArgs& a, int D, bool inter, unsigned grid, hipStream_t stream) {
-    if (D == 32) return rope_launch<T, 32>(a, inter, grid, stream);
-    if (D == 64) return rope_launch<T, 64>(a, inter, grid, stream);
-    return rope_launch<T, 128>(a, inter, grid, stream);
+int rope_by_dim(const RopeArgs& a, int D, bool inter, hipStream_t stream) {
+    if (D == 32) return rope_by_size<T, 32>(a, inter, stream);
+    if (D == 64) return rope_by_size<T, 64>(a, inter, stream);
+    return rope_by_size<T, 128>(a, inter, stream);
 }
 
 }  // namespace
@@ -191,13 +204,9 @@ extern "C" int rag_enc_qk_norm_rope_dev(const void* d_qkv, int64_t qkv_stride, c
     a.n_tokens = n_tokens; a.n_rows = n_kv_rows;
     a.rot = rot_dim; a.hq = n_q_heads; a.hkv = n_kv_heads; a.heads = n_q_heads + (d_v_out ? 2 : 1) * n_kv_heads;
     a.eps = eps;
-    const int per_wave = 64 / (head_dim / 8) * ROPE_U;
-    a.chunks = (a.heads + per_wave - 1) / per_wave;
     RAG_REQUIRE(n_tokens < (1ll << 40), RAG_ELIMIT, "%s: too many tokens", me);
-    const int64_t grid = ceil_div64(n_tokens * a.chunks, ROPE_NT / 64);
-    RAG_REQUIRE(grid < (1ll << 24), RAG_ELIMIT, "%s: too many tokens", me);
     hipStream_t stream = (hipStream_t)stream_;
-    if (dtype == RAG_DTYPE_F32) return rope_by_dim<float>(a, head_dim, interleaved != 0, (unsigned)grid, stream);
-    if (dtype == RAG_DTYPE_BF16) return rope_by_dim<bf16>(a, head_dim, interleaved != 0, (unsigned)grid, stream);
-    return rope_by_dim<f16>(a, head_dim, interleaved != 0, (unsigned)grid, stream);
+    if (dtype == RAG_DTYPE_F32) return rope_by_dim<float>(a, head_dim, interleaved != 0, stream);
+    if (dtype == RAG_DTYPE_BF16) return rope_by_dim<bf16>(a, head_dim, interleaved != 0, stream);
+    return rope_by_dim<f16>(a, head_dim, interleaved != 0, stream);
 }

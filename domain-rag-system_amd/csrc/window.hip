@@ -1021,7 +1021,7 @@ Plan plan_of(int64_t total_q, int n_seq, int max_q, int max_k, int hq, int hkv, 
     // launch; the few-query kernel spreads them too but reads them once per 64 rows, with narrower matrix operands.  The
     // constants are fitted to the kernels' times over 197 sizes a type and head size (1 to 32 sequences, 9 to 1500 queries, 600 to
     // 16384 keys); the chosen times are 1 % over the best of the three on average, without the spans 30 %.  E.g. head size 128,
-    // bf16, 16 heads on 8, 4 sequences of 200 queries on 4096 keys: few 102 us, spans 58, tiles 91; of 9 queries: 21, 26, 85.
+    // bf16, 16 heads on 8, 4 sequences of 200 queries on 4096 keys: few 102 us, spans 58, tiles 91; of 9 queries: 24, 23, 85.
     static const double few_tile[2][3] = {{1.0, 1.0, 1.7}, {1.0, 2.4, 3.4}};            // of 17 to 32 rows
     static const double one_tile[2][3] = {{0.9, 0.9, 1.0}, {0.9, 1.5, 1.8}}, all_tiles[2][3] = {{0.7, 0.7, 1.07}, {0.7, 1.3, 1.8}};
     static const int on_cu[2][3] = {{4, 3, 2}, {4, 2, 1}};   // workgroups of the tile kernel

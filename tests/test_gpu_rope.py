@@ -206,3 +206,35 @@ def test_another_stream_and_a_replayed_graph():
         torch.cuda.synchronize()
         q0, k0, _ = _call(qkv, pos, inv, hq, hkv, gq, gq, False)
         assert torch.equal(q0, q2) and torch.equal(k0, k2), i
+
+
+@pytest.mark.parametrize('kind', list(TYPES))
+@pytest.mark.parametrize('t,hq,hkv,d,rot,inter,norm', [
+    (5000, 13, 4, 128, 128, False, True), (4999, 5, 3, 64, 40, True, True), (4400, 17, 16, 32, 32, False, False), (4097, 1, 1, 32, 16, True, True),
+    (4096, 1, 1, 32, 16, False, True)])
+def test_many_tokens(kind, t, hq, hkv, d, rot, inter, norm):
+    # more waves than a lane with one head each would have on the chip: four heads a lane, heads that end inside its four
+    import rag_hip
+    g, dt = _gen(t + d), TYPES[kind]
+    qkv = torch.randn((t, (hq + 2 * hkv) * d), generator=g, device=_dev()).to(dt)
+    pos = torch.randint(0, 1 << 17, (t,), generator=g, device=_dev(), dtype=torch.int32)
+    inv = rag_hip.rope_inv_freq(rot)
+    gq, gk = ((1 + 0.3 * torch.randn(d, generator=g, device=_dev())).to(dt) if norm else None for _ in range(2))
+    x = qkv.clone().view(t, hq + 2 * hkv, d)
+    rows = torch.randperm(t + 9, generator=g, device=_dev())[:t].to(torch.int64)
+    rows[5::7] = -1
+    k_out, v_out = (torch.full((t + 9, hkv, d), 3.0, dtype=dt, device=_dev()) for _ in range(2))
+    q, _, _ = _call(qkv, pos, inv, hq, hkv, gq, gk, inter, k_out=k_out, v_out=v_out, kv_row=rows)
+    kept = rows >= 0
+    k_ref, k_mag = _ref(x[:, hq:hq + hkv], pos, inv, gk, 1e-6, inter)
+    _close(q, *_ref(x[:, :hq], pos, inv, gq, 1e-6, inter))
+    _close(k_out[rows[kept]], k_ref[kept], k_mag[kept])
+    assert torch.equal(v_out[rows[kept]], x[:, hq + hkv:][kept])
+    other = torch.ones(t + 9, dtype=torch.bool, device=_dev())
+    other[rows[kept]] = False
+    assert bool((k_out[other] == 3.0).all()) and bool((v_out[other] == 3.0).all())
+    # in place
+    heads = qkv.view(t, hq + 2 * hkv, d)
+    _call(qkv, pos, inv, hq, hkv, gq, gk, inter, q_out=heads[:, :hq], k_out=heads[:, hq:hq + hkv])
+    assert torch.equal(heads[:, :hq], q) and torch.equal(heads[:, hq:hq + hkv][kept], k_out[rows[kept]])
+    assert torch.equal(heads[:, hq + hkv:], x[:, hq + hkv:])
