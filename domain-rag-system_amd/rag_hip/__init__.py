@@ -1261,17 +1261,18 @@ def _enc_code(dtype):
     return code
 
 
-_current = []                        # torch's own functions: current device, its current stream
+_current = None                      # torch's own functions: current device, its current stream
 
 
 def _here_and_stream(*tensors):
     """The current stream of the current GPU, after checking that every tensor given (None: skipped) is on that GPU."""
-    if not _current:
+    global _current
+    if _current is None:
         import torch
         torch.cuda.current_device()                          # (initialises the GPU; what it calls after that is four times as fast)
         raw = getattr(torch._C, '_cuda_getCurrentRawStream', None)          # (current_stream() builds an object around it: 4 us)
-        _current.extend((getattr(torch._C, '_cuda_getDevice', torch.cuda.current_device),
-                         raw if raw is not None else lambda d: torch.cuda.current_stream(d).cuda_stream))
+        _current = (getattr(torch._C, '_cuda_getDevice', torch.cuda.current_device),
+                    raw if raw is not None else lambda d: torch.cuda.current_stream(d).cuda_stream)
     device, stream = _current
     here = device()
     for t in tensors:

@@ -148,3 +148,25 @@ def test_weights_beyond_the_interface_are_refused():
     x = torch.zeros((1, 32), device='cuda')
     with pytest.raises(ValueError, match='2\\^31'):
         rag_hip.enc_linear4_dev(x, torch.zeros((1, 16), dtype=torch.uint8, device='cuda').expand(1 << 32, 16), torch.zeros((1, 1), device='cuda').expand(1 << 32, 1))
+
+
+def test_first_calls_of_many_threads():
+    # what the wrapper keeps of torch is set once, whichever thread comes first
+    import threading
+    import rag_hip
+    x, codes, scales, off, _ = _operands(3, 64, 128, 32, True, torch.float32, 5)
+    want = rag_hip.enc_linear4_dev(x, codes, scales, off)
+    torch.cuda.synchronize()
+    for _ in range(5):
+        rag_hip._current, got, start = None, [None] * 8, threading.Barrier(8)
+
+        def run(i):
+            start.wait()
+            got[i] = rag_hip.enc_linear4_dev(x, codes, scales, off)
+        threads = [threading.Thread(target=run, args=(i,)) for i in range(8)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        torch.cuda.synchronize()
+        assert all(y is not None and torch.equal(y, want) for y in got)
