@@ -1399,7 +1399,7 @@ def enc_attention_window_dev(q, k, v, cu_q, max_q_len, k_start=None, k_len=None,
         raise ValueError("the heads of a row of q must lie side by side")
     max_q_len, max_k_len, window_left, window_right, n_sinks = int(max_q_len), int(max_k_len), int(window_left), int(window_right), int(n_sinks)
     need = _window_workspace(tq, n_seq, max_q_len, max_k_len, hq, hkv, d, window_left, window_right, n_sinks, code)
-    work = torch.empty((need,), dtype=torch.uint8, device=q.device) if need > 0 else None
+    work = q.new_empty((need // (4 if code == DTYPE_F32 else 2),)) if need > 0 else None       # (need: a multiple of 8)
     check(lib().rag_enc_attention_window_dev(qp, qs if tq > 1 else hq * d, kp, krs, khs, vp, vrs, vhs, _flat(cu_q, torch.int32, 'cu_q'), tq,
                                              _flat(k_start, torch.int64, 'k_start'), _flat(k_len, torch.int32, 'k_len'), tk, n_seq,
                                              max_q_len, max_k_len, hq, hkv, d, d ** -0.5 if scale is None else scale, window_left,
