@@ -580,7 +580,7 @@ int rag_enc_qk_norm_rope_dev(const void* d_qkv, int64_t qkv_stride, const int32_
  * without k_start, max_q_len stands for max_k_len, here and in the workspace's size.
  * dtype bf16, fp16 (matrix cores, fp32 softmax and sums) or fp32; head_dim 32, 64 or 128; pointers and strides multiples
  * of 16 bytes, rows of k and v at most 32 MB apart; out must not overlap q, k or v.  workspace: rag_enc_attention_window_workspace() bytes for the same sizes (0:
- * may be NULL), 16-byte aligned, used by this call alone until it has run on its stream.                    */
+ * may be NULL), 16-byte aligned, used by this call alone until it has run on its stream; what it holds before does not matter. */
 int64_t rag_enc_attention_window_workspace(int64_t total_q, int32_t n_seq, int32_t max_q_len, int32_t max_k_len,
                                            int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
                                            int32_t window_left, int32_t window_right, int32_t n_sinks, int32_t dtype);
