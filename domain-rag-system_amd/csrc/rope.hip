@@ -9,11 +9,12 @@
 // Bytes bound: an element is read once, written once, and costs about fifteen instructions.  A head is D/8 lanes of a
 // wave; a lane owns two pieces of four dimensions which are rotated against each other, so the rotation needs no
 // exchange between lanes and the sum of squares only the D/8 lanes of the head.  Angles are the same for every head of
-// a token: a lane's four are computed once and used for all heads the wave takes.  They are reduced to a fraction of
+// a token: a lane computes one, takes its four from the others and uses them for all heads of the wave (four computed
+// by every lane: 16384 tokens 73 us for 69, 24 heads of 32 17.9 for 15.5).  They are reduced to a fraction of
 // a turn in 64 bits (a 32-bit product is off by 2^-24 of the angle itself, 0.002 radians at position 32768) and only
 // the sine and cosine of the remainder are taken in 32 bits, so there is no table to read or to size.
-// Measured: 16384 tokens of 32 query and 8 key heads of 128, bf16, 70.6 us, 4.75 TB/s (a large copy moves 4.7); 65536 tokens
-// of 16 and 8 heads of 128, half of each rotated, f16, 161 us, 5.0 TB/s; one token 2.8 us, of which an empty launch is 1.6.
+// Measured: 16384 tokens of 32 query and 8 key heads of 128, bf16, 69 us, 4.86 TB/s (a large copy moves 4.7); 65536 tokens
+// of 16 and 8 heads of 128, half of each rotated, f16, 156 us, 5.2 TB/s; one token 2.5 us, of which an empty launch is 1.6.
 #include "common.h"
 
 namespace {
@@ -72,16 +73,17 @@ __global__ __launch_bounds__(ROPE_NT) void qk_norm_rope_kernel(RopeArgs a, uint3
     const bool kv_ok = kv >= 0 && kv < a.n_rows;
     if (kv >= a.n_rows && chunk == 0 && lane == 0) rag_flag(fault, RAG_FAULT_KV_ROW);
 
+    // an angle a lane (at most 64), then the lane's four from those; beyond rot / 2: no turn
+    float my_co = 1.f, my_si = 0.f;
+    if (lane < a.rot / 2) {
+        const double turn = (double)a.pos[t] * 0.15915494309189533577 * a.inv_freq[lane];          // 1 / (2 pi)
+        sincospif(2.f * (float)(turn - rint(turn)), &my_si, &my_co);
+    }
     float co[4], si[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) { co[j] = 1.f; si[j] = 0.f; }
-    if (turns) {
-        const double at = (double)a.pos[t] * 0.15915494309189533577;      // 1 / (2 pi)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const double turn = at * a.inv_freq[4 * p + j];
-            sincospif(2.f * (float)(turn - rint(turn)), &si[j], &co[j]);
-        }
+    for (int j = 0; j < 4; ++j) {
+        co[j] = __shfl(my_co, 4 * p + j, 64);
+        si[j] = __shfl(my_si, 4 * p + j, 64);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -153,13 +155,13 @@ int rope_launch(RopeArgs a, bool inter, hipStream_t stream) {
     return RAG_OK;
 }
 
-// One head a lane while that leaves the chip no more than 16 waves a compute unit: less to do one after the other (16 + 8
-// heads of 128, bf16: one token 2.8 us, with four heads 4.3, 512 tokens 4.0 and 5.2).  Beyond that four: more bytes in
-// flight and the angles for four heads at once (8192 tokens 23.7 us, with one head 30.5).
+// One head a lane while the waves are on the chip at once, 32 a compute unit: less to do one after the other (16 + 8 heads
+// of 128, bf16: one token 2.6 us, with four heads 4.2, 512 tokens 3.5 and 5.1, 1024 5.2 and 5.7).  Beyond that four: more bytes in
+// flight and the angles for four heads at once (2048 tokens 7.8 us, with one head 8.2, 8192 22.5 and 25.2).
 template <typename T, int D>
 int rope_by_size(const RopeArgs& a, bool inter, hipStream_t stream) {
     const int64_t waves = a.n_tokens * ((a.heads + 512 / D - 1) / (512 / D));
-    return waves <= 4096 ? rope_launch<T, D, 1>(a, inter, stream) : rope_launch<T, D, 4>(a, inter, stream);
+    return waves <= 8192 ? rope_launch<T, D, 1>(a, inter, stream) : rope_launch<T, D, 4>(a, inter, stream);
 }
 
 template <typename T>

@@ -211,7 +211,8 @@ def test_another_stream_and_a_replayed_graph():
 @pytest.mark.parametrize('kind', list(TYPES))
 @pytest.mark.parametrize('t,hq,hkv,d,rot,inter,norm', [
     (5000, 13, 4, 128, 128, False, True), (4999, 5, 3, 64, 40, True, True), (4400, 17, 16, 32, 32, False, False), (4097, 1, 1, 32, 16, True, True),
-    (4096, 1, 1, 32, 16, False, True)])
+    (4096, 1, 1, 32, 16, False, True),
+    (8192, 1, 1, 32, 24, False, True), (8193, 1, 1, 32, 24, False, True)])
 def test_many_tokens(kind, t, hq, hkv, d, rot, inter, norm):
     # more waves than a lane with one head each would have on the chip: four heads a lane, heads that end inside its four
     import rag_hip
