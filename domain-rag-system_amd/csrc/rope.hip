@@ -120,22 +120,30 @@ __global__ __launch_bounds__(ROPE_NT) void qk_norm_rope_kernel(RopeArgs a, uint3
 #pragma unroll
             for (int j = 0; j < 4; ++j) { fa[j] *= inv * (float)ga[j]; fb[j] *= inv * (float)gb[j]; }
         }
-        v4 ya, yb;
-        if (INTER) {                                          // pairs (0, 1), (2, 3) of each piece
+        // Dimensions behind rot_dim stay as they are: a product with a sine of 0 would pass an infinity or a NaN on.
+        if (turns) {
+            float ra[4], rb[4];
+            if (INTER) {                                      // pairs (0, 1), (2, 3) of each piece
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                ya[2 * j] = (T)(fa[2 * j] * co[j] - fa[2 * j + 1] * si[j]);
-                ya[2 * j + 1] = (T)(fa[2 * j + 1] * co[j] + fa[2 * j] * si[j]);
-                yb[2 * j] = (T)(fb[2 * j] * co[2 + j] - fb[2 * j + 1] * si[2 + j]);
-                yb[2 * j + 1] = (T)(fb[2 * j + 1] * co[2 + j] + fb[2 * j] * si[2 + j]);
-            }
-        } else {
+                for (int j = 0; j < 2; ++j) {
+                    ra[2 * j] = fa[2 * j] * co[j] - fa[2 * j + 1] * si[j];
+                    ra[2 * j + 1] = fa[2 * j + 1] * co[j] + fa[2 * j] * si[j];
+                    rb[2 * j] = fb[2 * j] * co[2 + j] - fb[2 * j + 1] * si[2 + j];
+                    rb[2 * j + 1] = fb[2 * j + 1] * co[2 + j] + fb[2 * j] * si[2 + j];
+                }
+            } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                ya[j] = (T)(fa[j] * co[j] - fb[j] * si[j]);
-                yb[j] = (T)(fb[j] * co[j] + fa[j] * si[j]);
+                for (int j = 0; j < 4; ++j) {
+                    ra[j] = fa[j] * co[j] - fb[j] * si[j];
+                    rb[j] = fb[j] * co[j] + fa[j] * si[j];
+                }
             }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { fa[j] = ra[j]; fb[j] = rb[j]; }
         }
+        v4 ya, yb;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { ya[j] = (T)fa[j]; yb[j] = (T)fb[j]; }
         if (is_q || kv_ok) {
             *reinterpret_cast<v4*>(dst + off_a) = ya;
             *reinterpret_cast<v4*>(dst + off_b) = yb;

@@ -239,3 +239,41 @@ def test_many_tokens(kind, t, hq, hkv, d, rot, inter, norm):
     _call(qkv, pos, inv, hq, hkv, gq, gk, inter, q_out=heads[:, :hq], k_out=heads[:, hq:hq + hkv])
     assert torch.equal(heads[:, :hq], q) and torch.equal(heads[:, hq:hq + hkv][kept], k_out[rows[kept]])
     assert torch.equal(heads[:, hq + hkv:], x[:, hq + hkv:])
+
+
+@pytest.mark.parametrize('kind', list(TYPES))
+@pytest.mark.parametrize('inter', [False, True])
+@pytest.mark.parametrize('t,d,rot', [(3, 32, 0), (3, 64, 24), (9000, 128, 64), (9000, 32, 8), (2, 128, 0)])
+def test_an_infinity_outside_the_rotation_stays_where_it_is(kind, inter, t, d, rot):
+    # without a norm, dimensions from rot_dim on are copied: what one of them holds does not reach another
+    import rag_hip
+    dt, hq, hkv = TYPES[kind], 3, 2
+    qkv = torch.randn((t, (hq + 2 * hkv) * d), generator=_gen(d + rot), device=_dev()).to(dt)
+    pos = torch.arange(t, dtype=torch.int32, device=_dev())
+    inv = rag_hip.rope_inv_freq(rot) if rot else None
+    want_q, want_k, _ = _call(qkv, pos, inv, hq, hkv, None, None, inter)
+    bad = qkv.clone().view(t, hq + 2 * hkv, d)
+    for i, x in enumerate((float('inf'), float('nan'), -float('inf'))):
+        bad[i % t, i % hq, rot + (5 + 3 * i) % (d - rot)] = x          # one dimension of a query head each,
+        bad[(i + 1) % t, hq + i % hkv, rot + 2 * i] = x                 # of a key head,
+        bad[t - 1, :hq + hkv, d - 1 - i] = x                            # and the last ones of all
+    q, k, _ = _call(bad.view(t, -1), pos, inv, hq, hkv, None, None, inter)
+    for got, want, x in ((q, want_q, bad[:, :hq]), (k, want_k, bad[:, hq:hq + hkv])):
+        assert torch.equal(got[..., :rot], want[..., :rot])
+        torch.testing.assert_close(got[..., rot:], x[..., rot:], rtol=0, atol=0, equal_nan=True)
+
+
+@pytest.mark.parametrize('kind', list(TYPES))
+@pytest.mark.parametrize('inter', [False, True])
+def test_an_infinity_under_the_norm(kind, inter):
+    # x / inf: the head's finite dimensions become 0, the infinite one infinity / infinity; rotated, it takes its pair with it
+    import rag_hip
+    dt, t, d, rot = TYPES[kind], 2, 64, 16
+    qkv = torch.randn((t, 3 * d), generator=_gen(1), device=_dev()).to(dt)
+    qkv[0, 40] = float('inf')
+    qkv[1, 3] = -float('inf')
+    ones = torch.ones(d, dtype=dt, device=_dev())
+    q, _, _ = _call(qkv, torch.arange(1, 3, dtype=torch.int32, device=_dev()), rag_hip.rope_inv_freq(rot), 1, 1, ones, ones, inter)
+    nan = torch.zeros((t, d), dtype=torch.bool, device=_dev())
+    nan[0, 40] = nan[1, 3] = nan[1, 2 if inter else 3 + rot // 2] = True
+    assert torch.equal(torch.isnan(q[:, 0]), nan) and float(q[:, 0][~nan].abs().max()) == 0.0
