@@ -117,6 +117,46 @@ template <> struct ScalePair<float> {
     __device__ static void split(type p, float& s, float& o) { s = p.x; o = p.y; }
 };
 
+// The sums of x times 16 + code, and 16 scales, can leave the range of fp32 (x of 1e35 and more, scales of 1e37) where x times
+// whole weights does not.  So what is not finite is computed again from those, by a wave: finite_row tells whether x itself
+// is the reason, which leaves the value as it is (n 16384, k 8192, bf16: 13 rows, a NaN in one of them, 28 us; 64 rows with a NaN each
+// 220, without 43).  With neither, the look at the sums costs 0.1 us.
+template <typename T>
+__device__ bool finite_row(const Lin4Args& a, int64_t m, int lane) {
+    const T* x = reinterpret_cast<const T*>(a.x) + m * a.x_stride;
+    struct alignas(16) Piece { T v[8]; };
+    for (int c = 8 * lane; __any(c < a.k); c += 512) {       // (rows are whole pieces)
+        bool good = true;
+        if (c < a.k) {
+            const Piece p = *reinterpret_cast<const Piece*>(x + c);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) good &= isfinite((float)p.v[e]);
+        }
+        if (!__all(good)) return false;
+    }
+    return true;
+}
+template <typename T>
+__device__ float whole_product(const Lin4Args& a, int64_t m, int64_t n, int lane) {
+    const T* x = reinterpret_cast<const T*>(a.x) + m * a.x_stride;
+    const uint8_t* codes = a.codes + n * (a.k / 2);
+    const T* scales = reinterpret_cast<const T*>(a.scales) + n * (a.k / a.group);
+    const T* offsets = reinterpret_cast<const T*>(a.offsets) + n * (a.k / a.group);
+    float sum = 0.f;
+    for (int c = 8 * lane; c < a.k; c += 512) {              // (eight columns never cross a group)
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(codes + c / 2);
+        const float s = (float)scales[c / a.group], o = a.offsets != nullptr ? (float)offsets[c / a.group] : 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float code = (float)(w >> (4 * e) & 15u);
+            sum = fmaf((float)x[c + e], a.offsets != nullptr ? fmaf(s, code, o) : s * (code - 8.f), sum);
+        }
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
+    return sum;
+}
+
 // A workgroup takes 16 * RT rows of the weights and 16 * MT rows of x; its waves take the 128-column blocks of the weights
 // in turn and add their sums up through LDS.  x is the A operand of v_mfma_f32_16x16x32, the codes are the B operand, so a
 // lane ends with its own weight row's sums for four rows of x, and a group's scale is one value per lane.
@@ -131,7 +171,8 @@ template <> struct ScalePair<float> {
 // n 16384, k 8192, group 64, m 1: codes alone 12.7 us, with scales loaded by lane 26.7 us).
 //
 // The operand holds 16 + code.  With c = sum x (16 + code) and X = sum x over a group (the same product with ones),
-// sum x w = scale c + (offset - 16 scale) X.
+// sum x w = scale c + (offset - 16 scale) X.  These sums are some five times larger than what is left of them (fp32 x: error 4e-7
+// of the result's size, with whole weights 2e-7), and may overflow where it does not: see whole_product.
 //
 // The loads of the wave's next block are issued before the products of this one.  Loads return in order: x, which comes from the L2, is
 // asked for before the codes of the next block, which come from memory, or with its own block (MT == 1).
@@ -364,8 +405,27 @@ __global__ __launch_bounds__((64 * max_waves<T, RT>())) void linear4_kernel(Lin4
     for (int i = tid; i < RT * MT * 64; i += (int)blockDim.x) {
         f32x4 sum = part[i];
         for (int v = 1; v < waves; ++v) sum += part[v * RT * MT * 64 + i];
-        const int n = ((int)blockIdx.x * RT + i / (MT * 64)) * 16 + (i & 15);
-        const int64_t m = m0 + 16 * ((i / 64) % MT) + 4 * ((i & 63) >> 4);
+        const int n0 = ((int)blockIdx.x * RT + i / (MT * 64)) * 16, n = n0 + (i & 15);
+        const int64_t m1 = m0 + 16 * ((i / 64) % MT), m = m1 + 4 * ((i & 63) >> 4);
+        const f32x4 none = sum - sum;                        // (0 where finite; the lanes of a wave are at the same n0 and m1)
+        const bool bad = !(none[0] + none[1] + none[2] + none[3] == 0.f) && n < a.n;
+        if (__builtin_expect(__any(bad), 0)) {
+#pragma unroll 1
+            for (int row = 0; row < 16 && m1 + row < a.m; ++row) {
+                float mine = sum[0];
+#pragma unroll
+                for (int j = 1; j < 4; ++j) mine = (row & 3) == j ? sum[j] : mine;
+                uint64_t rest = __ballot(bad && lane >> 4 == row >> 2 && !isfinite(mine));
+                if (rest == 0 || !finite_row<T>(a, m1 + row, lane)) continue;
+                for (; rest != 0; rest &= rest - 1) {
+                    const int from = __builtin_ctzll(rest);
+                    const float again = whole_product<T>(a, m1 + row, n0 + (from & 15), lane);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (lane == from && (row & 3) == j) sum[j] = again;
+                }
+            }
+        }
         if (n >= a.n) continue;
         const float bias = a.bias ? (float)reinterpret_cast<const T*>(a.bias)[n] : 0.f;
 #pragma unroll

@@ -596,7 +596,8 @@ int rag_enc_attention_window_dev(const void* d_q, int64_t q_stride, const void* 
  * the row, column 2i + 1 in its high half; scales, offsets [n][k / group], bias [n] (or NULL) of x's type (bf16, fp16 or
  * fp32).  Made for the few rows of one query (the weights are read once per 16 or 32 rows of x).  fp32 sums.
  * group 32, 64 or 128, k < 2^26 a multiple of it, n < 2^28, m up to 2 million; x, its rows and the codes aligned to 16 bytes, rows of
- * x at most 32 MB apart; y must not overlap x.  A row of x that holds an infinity or a NaN gives infinities or NaN.   */
+ * x at most 32 MB apart; y must not overlap x.  A row of x that holds an infinity or a NaN gives infinities or NaN;
+ * finite rows give what fp32 sums of x times w give, also where sums of x and codes alone would overflow.         */
 int rag_enc_linear4_dev(const void* d_x, int64_t x_stride, const uint8_t* d_codes, const void* d_scales,
                         const void* d_offsets, const void* d_bias, int64_t m, int32_t n, int32_t k, int32_t group,
                         int32_t dtype, void* d_y, int64_t y_stride, void* stream);

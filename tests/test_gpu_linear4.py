@@ -170,3 +170,44 @@ def test_first_calls_of_many_threads():
             t.join()
         torch.cuda.synchronize()
         assert all(y is not None and torch.equal(y, want) for y in got)
+
+
+# every tile of the kernel, x as operands and by rows
+LARGE = [(1, 40, 128, 128), (3, 17, 1024, 128), (13, 600, 640, 128), (2, 5000, 256, 64), (13, 5000, 256, 32), (40, 5000, 384, 64), (64, 384, 1536, 128),
+         (200, 5000, 256, 128)]
+
+
+@pytest.mark.parametrize('kind', ['bf16', 'f32'])
+@pytest.mark.parametrize('m,n,k,group', LARGE)
+@pytest.mark.parametrize('offsets', [False, True])
+def test_finite_products_of_large_values(kind, m, n, k, group, offsets):
+    # x of 1e37 and weights of some thousandths: the sum of all magnitudes stays below 1e38, while x times a code of 24 does not
+    import rag_hip
+    x, codes, scales, off, bias = _operands(m, n, k, group, offsets, TYPES[kind], m + k)
+    want = rag_hip.enc_linear4_dev(x, codes, scales * 0.01, off * 0.01 if offsets else None, bias)
+    large = list(range(0, m, 3))
+    x[large] *= 1e37
+    scales, off = scales * 0.01, off * 0.01 if offsets else None
+    c, s, o = _weights(codes, scales, off)
+    assert float((x.double().abs() @ (c * s + o).abs().t()).max()) < 2e38
+    y = rag_hip.enc_linear4_dev(x, codes, scales, off, bias)
+    assert bool(torch.isfinite(y).all())
+    _check(y, x, codes, scales, off, bias)
+    rest = [i for i in range(m) if i % 3]
+    assert torch.equal(y[rest], want[rest])
+
+
+@pytest.mark.parametrize('kind', ['bf16', 'f32'])
+@pytest.mark.parametrize('offsets', [False, True])
+def test_finite_products_of_large_scales(kind, offsets):
+    # weights up to 2e38, whose scale times 24, or offset minus 16 scales, is beyond the type
+    import rag_hip
+    x, codes, scales, off, bias = _operands(5, 70, 256, 64, offsets, TYPES[kind], 3)
+    x, scales = x * 1e-4, scales * 2e38 * 2
+    if offsets:
+        off = off * 0.5e38 - 8 * scales
+    c, s, o = _weights(codes, scales, off)
+    assert float((c * s + o).abs().max()) < 3e38
+    y = rag_hip.enc_linear4_dev(x, codes, scales, off, bias)
+    assert bool(torch.isfinite(y).all())
+    _check(y, x, codes, scales, off, bias)
