@@ -211,3 +211,19 @@ def test_finite_products_of_large_scales(kind, offsets):
     y = rag_hip.enc_linear4_dev(x, codes, scales, off, bias)
     assert bool(torch.isfinite(y).all())
     _check(y, x, codes, scales, off, bias)
+
+
+@pytest.mark.parametrize('m,n,k,group', [(1, 1152, 384, 64), (16, 300, 256, 32), (40, 5000, 1024, 64), (3, 500, 4096, 128), (200, 129, 640, 128), (9, 4111, 8192, 32)])
+@pytest.mark.parametrize('offsets', [False, True])
+def test_float32_keeps_24_bits_of_x(m, n, k, group, offsets):
+    # The worst-case tolerance above is too wide to tell 24 bits of x from 16, so the root-mean-square error is held to the root
+    # of the summed squares of what is added up (x times code + 16, x times the offset less 16 scales).  In half steps of that,
+    # 2^-24: a sum over 32 columns is at most some 36 roundings, each uniform (1 / sqrt(3)), 3.5, and again as many of the
+    # offsets' part, which is two thirds as large; two multiply-adds into a sum that grows over up to 64 steps: 4.6; together below
+    # 6.5.  One part of x less leaves 22 to 79 (computed with the parts in 64 bits at these sizes), two less over 7000.
+    import rag_hip
+    x, codes, scales, off, _ = _operands(m, n, k, group, offsets, torch.float32, 3 * m + k)
+    c, s, o = _weights(codes, scales, off)
+    err = rag_hip.enc_linear4_dev(x, codes, scales, off).double() - x.double() @ (c * s + o).t()
+    square = x.double() ** 2 @ (((c + 16) * s) ** 2 + (o - 16 * s) ** 2).t()
+    assert float(err.pow(2).mean().sqrt()) <= 8 * 2.0 ** -24 * float(square.mean().sqrt())

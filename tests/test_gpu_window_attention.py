@@ -544,3 +544,32 @@ def test_pieces_of_a_text_in_a_captured_graph():
         torch.cuda.synchronize()
         assert torch.equal(out, want), n
         _check(want, q, k, v, [nq], [(0, n)], -1, 0, 0, d ** -0.5)
+
+
+@pytest.mark.parametrize('hq,hkv,d', [(2, 2, 32), (4, 2, 64), (2, 1, 128)])
+@pytest.mark.parametrize('q_lens,k_lens,right', [([300, 600], None, -1), ([300, 600], None, 0), ([64, 64, 60], [2049, 700, 2000], 0), ([1, 3, 2], [4000, 300, 2500], 0)])
+def test_float32_keeps_24_bits(hq, hkv, d, q_lens, k_lens, right):
+    # The worst-case tolerance above is too wide to tell products of all 24 bits from less, so the root-mean-square error is held to
+    # the root of the summed squares of what is added up (weight times value).  In half steps of that, 2^-24: a score of
+    # magnitude 1 is at most d / 16 * 6 * 4 = 192 roundings, each uniform (1 / sqrt(3)), 8; its exponential with the
+    # multiply-add in front of it 5; the sums of weights and of weighted values grow over nk / 16 * 6 roundings, at most 0.9
+    # sqrt(nk) together.  One of the six products of parts left out gives 250 to 380 (computed with the parts in 64 bits).
+    import rag_hip
+    g = _gen(d + sum(q_lens))
+    k_rows = sum(q_lens if k_lens is None else k_lens)
+    q = torch.randn((sum(q_lens), hq, d), generator=g, device=_dev())
+    k, v = (torch.randn((k_rows, hkv, d), generator=g, device=_dev()) for _ in range(2))
+    kw = {}
+    if k_lens is not None:
+        kw = dict(k_start=_cu(k_lens)[:-1].long(), k_len=torch.tensor(k_lens, dtype=torch.int32, device=_dev()), max_k_len=max(k_lens))
+    got = rag_hip.enc_attention_window_dev(q, k, v, _cu(q_lens), max(q_lens), window_right=right, **kw).view(-1, hq, d).double()
+    at = k0 = 0
+    for nq, nk in zip(q_lens, q_lens if k_lens is None else k_lens):
+        hidden = torch.arange(nk, device=_dev())[None, :] > torch.arange(nk - nq, nk, device=_dev())[:, None]
+        for h in range(hq):
+            kk, vv = k[k0:k0 + nk, h // (hq // hkv)].double(), v[k0:k0 + nk, h // (hq // hkv)].double()
+            s = q[at:at + nq, h].double() @ kk.t() * d ** -0.5
+            w = torch.softmax(s.masked_fill(hidden, -math.inf) if right == 0 else s, dim=1)
+            err, square = got[at:at + nq, h] - w @ vv, w ** 2 @ vv ** 2
+            assert float(err.pow(2).mean().sqrt()) <= (16 + nk ** 0.5) * 2.0 ** -24 * float(square.mean().sqrt()), (nq, nk, h)
+        at, k0 = at + nq, k0 + nk
