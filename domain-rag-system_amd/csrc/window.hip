@@ -61,7 +61,10 @@ __device__ __forceinline__ Seen seen_by(const WinArgs& a, int p, int nk) {
     return w;
 }
 
-// One wave, one query row of one head.  Reads no key and no value that the query does not see.
+__device__ __forceinline__ bool not_finite(float x) { return !(fabsf(x) < INFINITY); }
+
+// One wave, one query row of one head.  Reads no key and no value that the query does not see, and keeps the mean of the values
+// so far instead of their sum, which may be beyond the type's range where the mean is not.
 template <typename T, int D>
 __device__ void attend_row(const WinArgs& a, const Seq& sq, int j, int head, int lane) {
     typedef typename Vec<T, 8>::type v8;
@@ -98,14 +101,15 @@ __device__ void attend_row(const WinArgs& a, const Seq& sq, int j, int head, int
         float sum = lane < n ? p : 0.f;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
-        const float alpha = exp2f(m - top);
-        l = l * alpha + sum;
-        o0 *= alpha;
-        o1 *= alpha;
+        const float l_old = l * exp2f(m - top);
+        l = l_old + sum;
         m = m_new;
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+        o0 *= l_old * inv;
+        o1 *= l_old * inv;
         for (int i = 0; i < n; i += PARTS) {
             const int mine = i + part;
-            const float pi = __shfl(p, min(mine, 63), 64);
+            const float pi = __shfl(p * inv, min(mine, 63), 64);
             if (mine < n) {
                 const int key = base + mine < w.s ? base + mine : base + mine - w.s + w.lo;
                 const T* vr = v + (int64_t)key * a.v_row + d0;
@@ -118,9 +122,8 @@ __device__ void attend_row(const WinArgs& a, const Seq& sq, int j, int head, int
     for (int o = DL; o < 64; o <<= 1) { o0 += __shfl_xor(o0, o, 64); o1 += __shfl_xor(o1, o, 64); }
     if (part == 0) {
         T* dst = reinterpret_cast<T*>(a.out) + (sq.q0 + j) * a.out_stride + (int64_t)head * D + d0;
-        const float inv = total > 0 ? 1.f / l : 0.f;
-        dst[0] = (T)(total > 0 ? o0 * inv : 0.f);
-        dst[1] = (T)(total > 0 ? o1 * inv : 0.f);
+        dst[0] = (T)(total == 0 ? 0.f : l > 0.f ? o0 : NAN);  // (l: 0 where every score is -infinity, NaN where one is)
+        dst[1] = (T)(total == 0 ? 0.f : l > 0.f ? o1 : NAN);
     }
 }
 
@@ -262,8 +265,9 @@ constexpr float LAG = 8.f;           // the maximum may lag behind by this power
 // SPANS: the rows are those of a key/value head (row = query * group + head of the group), the keys are cut as in FewArgs; 4
 // sequences of 64 queries, 32 heads of 128 on 8, 4000 to 16000 keys: 72 us (the few-query kernel 165, without spans 250).
 // Masked scores are -infinity; a tile that every query of the wave sees whole needs no mask, one that none sees is left
-// out.  Where keys or values hold infinities or NaN, 0 * infinity spoils rows that do not see them: every row that ends as
-// NaN is computed again by attend_row, which reads only what the row sees.
+// out.  Where keys or values hold infinities or NaN, 0 * infinity spoils rows that do not see them, and sums of values of
+// 1e36 and more may overflow where their mean does not: every row that does not end finite is computed again by attend_row, which
+// reads only what the row sees.
 // Bound by the matrix cores and the exponentials together: 16384 tokens, 16 heads of 128 on 8, window 4096: 0.48-0.50 ms,
 // 0.97-1.0 PFLOP/s (a library product of 8192^3 reaches 1.2); head size 64, no window: 0.36 ms for 2 x 8192, 0.77; float32:
 // 167 to 180 TFLOP/s, 1.0 to 1.1 PFLOP/s of bf16 products (a library product in fp32 reaches 0.15).
@@ -572,7 +576,7 @@ __global__ __launch_bounds__(256, (Image<E, D>::WAVES)) void window_tile_kernel(
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             o[dt][i] = any_seen ? o[dt][i] * inv : 0.f;
-            bad |= o[dt][i] != o[dt][i];
+            bad |= not_finite(o[dt][i]);
         }
     const uint64_t bad64 = __ballot(bad && row_on);
     const uint32_t bad_rows = (uint32_t)bad64 | (uint32_t)(bad64 >> 32);
@@ -627,6 +631,9 @@ template <typename E, int D> struct FewImage {
     static constexpr int BYTES = KT * ROWB;
     static constexpr int NW = 4;                             // waves
     static constexpr size_t lds(int rows) { return (size_t)NW * (4 * BYTES + rows * 8); }
+    // waves a SIMD that the LDS leaves room for (kept by the registers too: 23 us for 26 at head size 32 in float32, 64 x 4 queries,
+    // window 500), not where 64 rows would spill
+    static constexpr int waves(int rows) { return rows <= 32 ? (int)((160 << 10) / (lds(rows) + 1024)) : 1; }
     __device__ static int k_swizzle(int row) { return rows_swizzle(PIECES, row); }
     // 16 bits: 8 neighbouring rows x 2 neighbouring pieces; 32 bits: rows 4 apart, 4 pieces
     __device__ static int v_swizzle(int row) {
@@ -711,7 +718,7 @@ __device__ void join_row(const WinArgs& a, const FewArgs& f, const Seq& sq, int 
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         const float x = any_seen ? sum[e] * inv : 0.f;
-        bad |= x != x;
+        bad |= not_finite(x);
         v[e] = (E)x;
     }
     if (__any(bad)) attend_row<E, D>(a, sq, j, head, lane);
@@ -719,7 +726,7 @@ __device__ void join_row(const WinArgs& a, const FewArgs& f, const Seq& sq, int 
 }
 
 template <typename E, int D, int QT>
-__global__ __launch_bounds__(64 * (FewImage<E, D>::NW)) void window_few_kernel(WinArgs a, FewArgs f, uint32_t* fault) {
+__global__ __launch_bounds__(64 * (FewImage<E, D>::NW), (FewImage<E, D>::waves(16 * QT))) void window_few_kernel(WinArgs a, FewArgs f, uint32_t* fault) {
     typedef FewImage<E, D> I;
     constexpr int KT = I::KT, KB = KT / 16, DT = D / 16, KC = I::PIECES / 4, ROWS = 16 * QT, NW = I::NW;
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -936,7 +943,7 @@ __global__ __launch_bounds__(64 * (FewImage<E, D>::NW)) void window_few_kernel(W
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float x = any_seen ? sum[e] * inv : 0.f;
-                bad |= x != x;
+                bad |= not_finite(x);
                 v[e] = (E)x;
             }
             if (bad) atomicOr(&bad_rows[lr >> 5], 1u << (lr & 31));

@@ -573,3 +573,24 @@ def test_float32_keeps_24_bits(hq, hkv, d, q_lens, k_lens, right):
             err, square = got[at:at + nq, h] - w @ vv, w ** 2 @ vv ** 2
             assert float(err.pow(2).mean().sqrt()) <= (16 + nk ** 0.5) * 2.0 ** -24 * float(square.mean().sqrt()), (nq, nk, h)
         at, k0 = at + nq, k0 + nk
+
+
+@pytest.mark.parametrize('kind', ['bf16', 'f32'])
+@pytest.mark.parametrize('hq,hkv,d', [(2, 2, 32), (8, 2, 64), (4, 1, 128)])
+@pytest.mark.parametrize('q_lens,k_lens,left,right', [([1, 200, 77], None, -1, 0), ([300], None, 60, 60), ([1], [40], -1, 0), ([1], [2000], -1, 0),
+                                                      ([9, 3], [700, 2000], -1, 0), ([64, 50], [3000, 1800], -1, 0)])
+def test_values_near_the_end_of_the_range(kind, hq, hkv, d, q_lens, k_lens, left, right):
+    # values of 1e37 to 1e38: their weighted mean is as large, their sum with weights of up to 2^8, or of many keys, is beyond fp32
+    import rag_hip
+    dt, g = TYPES[kind], _gen(d + sum(q_lens))
+    k_rows = q_lens if k_lens is None else k_lens
+    q = (2 * torch.randn((sum(q_lens), hq, d), generator=g, device=_dev())).to(dt)
+    k = torch.randn((sum(k_rows), hkv, d), generator=g, device=_dev()).to(dt)
+    v = ((1 + 0.2 * torch.randn((sum(k_rows), hkv, d), generator=g, device=_dev())) * 4e37).to(dt)
+    v[:, :, ::3] *= -1
+    kw = {}
+    if k_lens is not None:
+        kw = dict(k_start=_cu(k_lens)[:-1].long(), k_len=torch.tensor(k_lens, dtype=torch.int32, device=_dev()), max_k_len=max(k_lens))
+    got = rag_hip.enc_attention_window_dev(q, k, v, _cu(q_lens), max(q_lens), window_left=left, window_right=right, **kw)
+    assert bool(torch.isfinite(got).all())
+    _check(got, q, k, v, q_lens, list(zip(_cu(k_rows).tolist(), k_rows)), left, right, 0, d ** -0.5)
