@@ -206,6 +206,11 @@ extern "C" int rag_enc_qk_norm_rope_dev(const void* d_qkv, int64_t qkv_stride, c
                 v_head_stride % 4 == 0, RAG_EINVAL, "%s: strides must be multiples of 4 elements", me);
     RAG_REQUIRE(qkv_stride >= (int64_t)(n_q_heads + 2 * n_kv_heads) * head_dim && q_stride >= (int64_t)n_q_heads * head_dim, RAG_EINVAL,
                 "%s: a row's stride is smaller than the row", me);
+    // (rows of every head may lie together, [head][row], so a stride may be smaller than a row of all heads, but not than a head)
+    const auto apart = [&](int64_t stride, int64_t n) { return n <= 1 || stride >= head_dim || stride <= -head_dim; };
+    RAG_REQUIRE(apart(k_row_stride, n_kv_rows) && apart(k_head_stride, n_kv_heads) &&
+                (!d_v_out || (apart(v_row_stride, n_kv_rows) && apart(v_head_stride, n_kv_heads))), RAG_EINVAL,
+                "%s: rows or heads of the keys or values overlap", me);
     RopeArgs a;
     a.qkv = d_qkv; a.pos = d_pos; a.gamma_q = d_gamma_q; a.gamma_k = d_gamma_k; a.inv_freq = d_inv_freq;
     a.q_out = d_q_out; a.k_out = d_k_out; a.v_out = d_v_out; a.kv_row = d_kv_row;

@@ -155,3 +155,16 @@ def test_workspace_of_many_sequences_and_heads_does_not_overflow():
                 for dtype in (0, 1):
                     for window in ((-1, -1, 0), (0, 0, 0), (big, big, big)):
                         assert f(big, big, max_q, max_k, hq, hkv, 128, *window, dtype) == 0       # they fill the chip: nothing is cut
+
+
+@pytest.mark.parametrize('kw', [dict(krs=0), dict(krs=-28), dict(khs=16), dict(khs=0), dict(v=True, vrs=0), dict(v=True, vhs=-16)])
+def test_rope_keys_and_values_that_overlap_are_refused(kw):
+    # an expanded tensor: all tokens, or all heads, would be written to the same place
+    keep, p = _buf(4096)
+    a = dict(t=2, rows=2, hq=1, hkv=2, stride=160, krs=64, khs=32, vrs=64, vhs=32)
+    a.update(kw)
+    if kw.get('v'):
+        a['v'] = p
+    rc, text = _rope(**a)
+    assert rc == -1 and 'overlap' in text
+    assert _rope(**{**a, 't': 0})[0] == 0
