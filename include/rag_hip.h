@@ -557,7 +557,8 @@ int rag_enc_add_layernorm_dev(const void* d_x, const void* d_residual, const voi
  * rot_dim on are normalised only.  Queries go to q_out (row = token, heads side by side); keys, and where v_out is given
  * the values as they are, go to row kv_row[token] (NULL: row = token) of arrays of n_kv_rows rows addressed by a row and
  * a head stride.  kv_row < 0: the token's key and value are not written; a row at or beyond n_kv_rows is not written
- * and flagged (RAG_FAULT_KV_ROW); no two tokens may name the same row.  fp32 arithmetic, one rounding per element.
+ * and flagged (RAG_FAULT_KV_ROW); no two tokens may name the same row, nor rows or heads overlap.  fp32 arithmetic, one rounding per element (the
+ * squares are summed in fp32 too: a head whose root mean square is above 1.6e18 becomes 0).
  * dtype bf16, fp16 or fp32; head_dim 32, 64 or 128; rot_dim a multiple of 8 up to head_dim (0: no rotation, pos and inv_freq may be NULL).
  * Pointers aligned to 4 elements, strides multiples of 4 elements.  q_out, k_out and v_out may be the query, key and
  * value columns of qkv itself (in place; kv_row NULL), otherwise they must not overlap it.                   */
