@@ -1435,6 +1435,8 @@ def quantize4(weight, group=64, dtype=None, symmetric=False):
         offsets = w.amin(dim=2).to(dtype)
         scales = ((w.amax(dim=2) - offsets.float()) / 15).clamp_min(0).to(dtype)
         low = offsets.float()
+    if not bool(torch.isfinite(scales).all()) or not bool(torch.isfinite(low).all()):
+        raise ValueError(f"the weight holds infinities or NaN, or its groups' scales or offsets are beyond {dtype}")
     step = scales.float()[:, :, None]
     code = torch.where(step > 0, (w - low[:, :, None]) / torch.where(step > 0, step, torch.ones_like(step)), torch.full_like(w, 8.0 if symmetric else 0.0))
     code = code.round().clamp(0, 15).to(torch.uint8).reshape(n, k // 2, 2)

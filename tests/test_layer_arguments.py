@@ -168,3 +168,21 @@ def test_rope_keys_and_values_that_overlap_are_refused(kw):
     rc, text = _rope(**a)
     assert rc == -1 and 'overlap' in text
     assert _rope(**{**a, 't': 0})[0] == 0
+
+
+@pytest.mark.parametrize('symmetric', [False, True])
+def test_quantize4_refuses_what_four_bits_cannot_hold(symmetric):
+    import rag_hip
+    w = torch.randn((4, 64), generator=torch.Generator().manual_seed(3))
+    for bad in (float('nan'), float('inf'), -float('inf')):
+        x = w.clone()
+        x[2, 40] = bad
+        with pytest.raises(ValueError, match='infinities or NaN'):
+            rag_hip.quantize4(x, 32, symmetric=symmetric)
+    with pytest.raises(ValueError, match='beyond torch.float16'):
+        rag_hip.quantize4(w * 1e6, 32, dtype=torch.float16, symmetric=symmetric)
+    x = w.clone()
+    x[1, 1], x[1, 2] = 3e38, -3e38                            # their difference, or 8 scales of 3e38 / 7, is beyond the type
+    with pytest.raises(ValueError, match='beyond torch.float32'):
+        rag_hip.quantize4(x, 32, symmetric=symmetric)
+    assert bool(torch.isfinite(rag_hip.quantize4(w * 1e4, 32, dtype=torch.float16, symmetric=symmetric)[1]).all())
