@@ -122,6 +122,43 @@ __device__ __forceinline__ double key_to_f64(uint64_t k) {
 }
 
 // ---------------------------------------------------------------------------------
+// device side: direct loads into LDS, lanes that share a matrix column
+// ---------------------------------------------------------------------------------
+
+// One wave-instruction of a direct-to-LDS load: lane l's 16 bytes at gbase + voff land at LDS byte lds_dst + 16 l (the
+// destination is wave-uniform base + lane order; only the source is per lane).  M0 carries the destination and belongs to the
+// compiler, so it is saved and restored inside the statement.  The compiler does not count this load: wait with s_waitcnt
+// vmcnt before reading.
+__device__ __forceinline__ void lds_dma16(uint32_t lds_dst, const void* gbase, uint32_t voff) {
+    unsigned keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep) : "v"(voff), "s"(lds_dst), "s"(gbase) : "memory");
+}
+
+// The two lanes of a query (32 apart) combine or trade registers with one cross-half swap instruction
+// (v_permlane32_swap: the upper half of the first operand changes places with the lower half of the second) instead
+// of a round trip through the LDS crossbar.
+__device__ __forceinline__ float both_halves_max(float v) {
+    const auto r2 = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r2[0]), __uint_as_float(r2[1]));
+}
+__device__ __forceinline__ float both_halves_sum(float v) {
+    const auto r2 = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r2[0]) + __uint_as_float(r2[1]);
+}
+// afterwards the lower lane holds (its a, the upper lane's a) and the upper lane (the lower lane's b, its b)
+__device__ __forceinline__ void trade_halves(uint32_t& a, uint32_t& b) {
+    const auto r2 = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+    a = r2[0];
+    b = r2[1];
+}
+__device__ __forceinline__ void trade_halves(float& a, float& b) {
+    const auto r2 = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    a = __uint_as_float(r2[0]);
+    b = __uint_as_float(r2[1]);
+}
+
+// ---------------------------------------------------------------------------------
 // device side: exact top-K threshold by most-significant-digit radix select
 //
 // Items are (key, row) pairs ordered lexicographically, larger = better; rows are

@@ -465,15 +465,6 @@ __global__ __launch_bounds__(WQ * WR * 64, 2) void dense_scan_kernel(DenseScanPa
     publish_strip<Cfg>(p, n_tiles, q0, wave, lane, strip, cnt_s, my_scratch);
 }
 
-// One wave-instruction of a direct-to-LDS load: lane l's 16 bytes at gbase + voff land at LDS byte
-// lds_dst + 16 l.  M0 carries the destination and belongs to the compiler, so it is saved and restored inside
-// the statement.  The compiler does not count this load: wait with s_waitcnt vmcnt before reading.
-__device__ __forceinline__ void lds_dma16(uint32_t lds_dst, const void* gbase, uint32_t voff) {
-    unsigned keep;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\ts_mov_b32 m0, %0"
-                 : "=&s"(keep) : "v"(voff), "s"(lds_dst), "s"(gbase) : "memory");
-}
-
 // LDS reads whose completion the SOURCE waits for, so that they can run a group of MFMAs ahead of their use (the
 // compiler issues a fragment read right before the MFMA that needs it and waits for it there).  lds_read16 only
 // issues; the value is defined after an lds_wait8<N> that names the register, with N = the number of LDS reads

@@ -104,29 +104,6 @@ template <> struct Vec8<float> {
 
 constexpr int LN_MAX_CHUNKS = 4;     // 8-element chunks per lane: hidden sizes up to 2048
 
-// The two lanes of a query (32 apart) combine or trade registers with one cross-half swap instruction
-// (v_permlane32_swap: the upper half of the first operand changes places with the lower half of the second) instead
-// of a round trip through the LDS crossbar.
-__device__ __forceinline__ float both_halves_max(float v) {
-    const auto r2 = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(r2[0]), __uint_as_float(r2[1]));
-}
-__device__ __forceinline__ float both_halves_sum(float v) {
-    const auto r2 = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return __uint_as_float(r2[0]) + __uint_as_float(r2[1]);
-}
-// afterwards the lower lane holds (its a, the upper lane's a) and the upper lane (the lower lane's b, its b)
-__device__ __forceinline__ void trade_halves(uint32_t& a, uint32_t& b) {
-    const auto r2 = __builtin_amdgcn_permlane32_swap(a, b, false, false);
-    a = r2[0];
-    b = r2[1];
-}
-__device__ __forceinline__ void trade_halves(float& a, float& b) {
-    const auto r2 = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
-    a = __uint_as_float(r2[0]);
-    b = __uint_as_float(r2[1]);
-}
-
 // LDS image of one head's keys and values:
 //   K   [kpad][D + 8]     rows padded by 16 B: the 16-byte operand reads of 32 keys spread over the banks
 //   V^T [D][kpad + 4]     rows padded by 8 B: 32 lanes read 8 B of 32 different d rows without conflict

@@ -80,14 +80,6 @@ struct FfnOutParams {
     float eps;
 };
 
-// One wave-instruction of a direct-to-LDS load: lane l's 16 bytes at gbase + voff land at LDS byte
-// lds_dst + 16 l.  M0 carries the destination and belongs to the compiler: saved and restored.  The compiler
-// does not count this load: wait with s_waitcnt vmcnt before reading.
-__device__ __forceinline__ void lds_dma16(uint32_t lds_dst, const void* gbase, uint32_t voff) {
-    unsigned keep;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\ts_mov_b32 m0, %0"
-                 : "=&s"(keep) : "v"(voff), "s"(lds_dst), "s"(gbase) : "memory");
-}
 // LDS reads whose completion the source waits for (counted lgkmcnt), so they can run several MFMAs ahead.
 template <int OFF, typename T>
 __device__ __forceinline__ void lds_read16(T& dst, uint32_t addr) {

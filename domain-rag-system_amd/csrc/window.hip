@@ -158,29 +158,6 @@ __device__ __forceinline__ int64_t part_at(const WinArgs& a, const FewArgs& f, c
 // ---- a tile of 128 queries of one head per workgroup ------------------------------------------------------
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-__device__ __forceinline__ float both_halves_max(float v) {
-    const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
-}
-__device__ __forceinline__ float both_halves_sum(float v) {
-    const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return __uint_as_float(p[0]) + __uint_as_float(p[1]);
-}
-__device__ __forceinline__ void trade_halves(uint32_t& a, uint32_t& b) {
-    const auto p = __builtin_amdgcn_permlane32_swap(a, b, false, false);
-    a = p[0];
-    b = p[1];
-}
-
-// One wave-instruction of a direct-to-LDS load: lane l's 16 bytes at gbase + voff land at LDS byte lds_dst + 16 l.  M0
-// carries the destination and belongs to the compiler, so it is saved and restored inside the statement.  The compiler
-// does not count this load: wait with s_waitcnt vmcnt before reading.
-__device__ __forceinline__ void lds_dma16(uint32_t lds_dst, const void* gbase, uint32_t voff) {
-    unsigned keep;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\ts_mov_b32 m0, %0"
-                 : "=&s"(keep) : "v"(voff), "s"(lds_dst), "s"(gbase) : "memory");
-}
-
 // 16 neighbouring rows of `pieces` 16-byte pieces, piece p of a row at place p ^ swizzle, cover all banks once at one p
 __device__ __forceinline__ int rows_swizzle(int pieces, int row) {
     return pieces >= 16 ? row & 15 : pieces == 8 ? (row >> 1) & 7 : (row >> 2) & 3;
