@@ -1,7 +1,7 @@
 // Products of a few rows with 4-bit weights: y[m][n] = sum_k x[m][k] w[n][k] + bias[n],
 // w[n][k] = scale[n][k / G] * code[n][k] + offset[n][k / G] (no offsets: scale * (code - 8)).  The dense layers of an
-// encoder for one query's tokens (MedicalEmbedder.encode of one text, reference src/indexing/embedder.py:65-71), where
-// reading the weights is what the layer costs.  gfx950 only.
+// encoder for one query's tokens, where reading the weights is what the layer costs (beside the 16-bit and fp32 layers of
+// MedicalEmbedder's encoders, reference src/indexing/embedder.py:65-71).  gfx950 only.
 // Measured, bf16, group 32, n 16383, k 8192 (75 MB): one token 20.7 us (3.6 TB/s; a large copy moves 4.7), 13 tokens 24 (147
 // TFLOP/s of products: the codes are unpacked by the vector units beside them, and the waves meet once per workgroup), 64
 // tokens 54; n 4096, k 4096, group 128 (8.9 MB): 5.3, 6.2 and 10.
@@ -97,7 +97,8 @@ template <> struct XFrag<float> {
     }
 };
 
-// (1024 threads leave 128 registers a lane: enough for one or two row tiles and 16-bit x)
+// The most waves an instance is compiled for: 1024 threads leave 128 registers a lane, enough for one row tile and 16-bit x, and for
+// two with x as operands; with x by rows 3 to 13 registers of two row tiles go to scratch, in launches of fewer waves too
 template <typename T, int RT> constexpr int max_waves() { return RT <= 2 && sizeof(T) == 2 ? 16 : 8; }
 
 // A group's scale and offset as one value
@@ -442,10 +443,10 @@ int linear4_by_group(Lin4Args a, hipStream_t stream) {
     int waves = 4;
     while (waves < max_waves<T, RT>() && waves < blocks && (int64_t)tiles * my * waves < 2048) waves *= 2;
     const dim3 grid((unsigned)tiles, (unsigned)my);
-    // at most 32 KB of scales at a time (24 where the images of x take 128)
+    // at most 32 KB of scales at a time (the images of x take at most 64)
     const int ng = 128 / a.group, row_bytes = 16 * RT * (int)sizeof(typename ScalePair<T>::type);
     const int images = ROWS ? waves * 16 * MT * 128 * (int)sizeof(T) : 0;
-    a.chunk = std::min(blocks, (images > 65536 ? 24576 : 32768) / (row_bytes * ng));
+    a.chunk = std::min(blocks, 32768 / (row_bytes * ng));
     a.image = (row_bytes * ((a.chunk * ng) | 1) + 1023) / 1024 * 1024;
     const size_t lds = std::max((size_t)a.image + images, (size_t)waves * MT * RT * 1024);
 #define RAG_LINEAR4_LAUNCH(G)                                                            \
@@ -465,10 +466,9 @@ int linear4_by_group(Lin4Args a, hipStream_t stream) {
 // rows and 64 rows of weights are more than the registers hold (n 16383, k 8192, m 24: 57 us, by rows 71).
 template <typename T, int MT, int RT>
 int linear4_tile(const Lin4Args& a, hipStream_t stream) {
-    if constexpr (sizeof(T) == 2 || RT < 4)
-        if (a.m > 4) return linear4_by_group<T, MT, RT, true>(a, stream);
-    if constexpr (sizeof(T) == 4 || RT < 4) return linear4_by_group<T, MT, RT, false>(a, stream);
-    return RAG_EINVAL;                                       // (64 rows of weights are for more than 16 of x)
+    if constexpr (sizeof(T) == 2 && RT == 4) return linear4_by_group<T, MT, RT, true>(a, stream);       // (64 rows of weights: more than 16 of x)
+    else if constexpr (RT == 4) return linear4_by_group<T, MT, RT, false>(a, stream);
+    else return a.m > 4 ? linear4_by_group<T, MT, RT, true>(a, stream) : linear4_by_group<T, MT, RT, false>(a, stream);
 }
 
 // The smallest tile with which the workgroups are on the chip at once, one per compute unit: x is read by each of them, so
