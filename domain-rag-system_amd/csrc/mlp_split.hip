@@ -120,8 +120,8 @@ __device__ __forceinline__ void split_f16(float x, f16& hi, f16& lo) {
     lo = (f16)(x - (float)hi);
 }
 
-// The same GELU on two values at once: the polynomial runs on the packed fp32 instructions (v_pk_fma_f32, ...),
-// half the issue slots of the scalar form; every operation is the scalar form's, so are the results.
+// The same GELU on two values at once, every operation and so every result the scalar form's.  (Two values an instruction, packed
+// fp32, are not emitted: see the Makefile; the loop takes as long either way, it is not bound by vector arithmetic.)
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) { return __builtin_elementwise_fma(a, b, c); }
 __device__ __forceinline__ f32x2 gelu_f32x2(f32x2 v) {

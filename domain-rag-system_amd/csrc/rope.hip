@@ -1,6 +1,6 @@
 // Norms of queries and keys for each head and the rotation by position, in one pass over the q|k|v projection's output,
-// with keys and values written where the attention reads them.  For encoders with rotary positions behind
-// MedicalEmbedder.encode (reference src/indexing/embedder.py:65-71).  gfx950 only.
+// with keys and values written where the attention reads them.  For encoders with rotary positions,
+// beside the BERT encoders of MedicalEmbedder (reference src/indexing/embedder.py:65-71), which have none.  gfx950 only.
 //
 //   n = x * gamma / sqrt(mean(x^2) + eps)        (gamma NULL: n = x)
 //   (n_a, n_b) -> (n_a cos - n_b sin, n_b cos + n_a sin),  angle = pos * inv_freq[i],

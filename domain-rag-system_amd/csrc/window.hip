@@ -1,7 +1,7 @@
 // Attention with a sliding window and a few first tokens that stay visible, over packed sequences whose keys may be
 // kept from earlier calls: self-attention of long documents in local layers, and the few new tokens of a query behind a
-// kept prefix.  For encoders with windowed layers behind MedicalEmbedder.encode (reference
-// src/indexing/embedder.py:65-71).  gfx950 only.
+// kept prefix.  For encoders with windowed layers, beside the BERT encoders of MedicalEmbedder (reference
+// src/indexing/embedder.py:65-71), which have none.  gfx950 only.
 //
 // Query j of a sequence with nq queries and nk keys stands at position p = nk - nq + j.  It sees key c (0 <= c < nk) if
 //   c - p <= right (right < 0: no limit)   and   (p - c <= left (left < 0: no limit)  or  c < n_sinks)
@@ -598,6 +598,8 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 // products, 16 * QT of them per workgroup, so that a key is read once for all of them.  Its waves take tiles of keys in
 // turn, each into its own two LDS buffers (no barrier until the end), and put their results together; a long text is cut
 // into spans of `span` tiles, one workgroup each, whose results the last of them puts together, or window_join_kernel.
+// Probabilities are rounded to a 16-bit type as above (float32 takes fp32 products, in which nothing is rounded); 64 rows of
+// float32 at head size 128 are more than the registers hold (44 go to scratch).
 // Bound by the bytes of the keys and values, 64 KB of them in flight per compute unit at head size 128: 16 tokens over 4000 to
 // 32768 kept rows of 8 heads in 0.19 ms, 5.1 TB/s (a large copy moves 4.7).  One token over a window of 1024: 8.4 us, of which the
 // launch, the loads of the arguments and the queries, and joining the spans are three quarters.
@@ -640,7 +642,10 @@ __device__ __forceinline__ float quarters_sum(float v) {
     return __uint_as_float(q[0]) + __uint_as_float(q[1]);
 }
 
-// Values that workgroups on other XCDs read or wrote in the same launch: past the L2, which is an XCD's own.
+// Values that workgroups on other XCDs read or wrote in the same launch: past the L2, which is an XCD's own.  Results and marks are
+// relaxed atomics of agent scope, which this chip writes through and reads past the L2s; their order is that of the hardware
+// (a store is counted done by s_waitcnt vmcnt when it has reached memory), not of the language, under which results and
+// marks would need a release and an acquire.  Those write back and drop a whole L2 (one token on 4096 keys 19 us for 9.1).
 __device__ __forceinline__ void store_through(void* p, float x, float y) {
     const uint64_t v = (uint64_t)__float_as_uint(y) << 32 | __float_as_uint(x);
     __hip_atomic_store(reinterpret_cast<uint64_t*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);

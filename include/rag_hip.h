@@ -545,8 +545,9 @@ int rag_enc_add_layernorm_dev(const void* d_x, const void* d_residual, const voi
                               int32_t dtype, void* d_out, void* stream);
 
 /* ---- pieces of encoders with rotary positions, windowed layers and 4-bit weights -------------------
- * What the dense encoders for long texts behind SentenceTransformer.encode (reference
- * src/indexing/embedder.py:65-71) have in place of learned positions and full attention.  The serving forms:
+ * What encoders for long texts have in place of the learned positions and full attention of the BERT encoders (reference
+ * src/indexing/embedder.py:65-71) that the other rag_enc_* calls serve.  They are called directly, from C or by their wrappers in
+ * rag_hip; MedicalEmbedder loads BERT encoders, which have no use for them.  The serving forms:
  * packed documents, and the few or single new tokens of a query behind keys that are kept between calls.   */
 
 /* Norms of queries and keys for each head and the rotation by position in one pass.  qkv: rows of qkv_stride elements,
@@ -577,9 +578,10 @@ int rag_enc_qk_norm_rope_dev(const void* d_qkv, int64_t qkv_stride, const int32_
  * out[row] = sum over the seen keys of softmax(scale q.k) v, head h with key/value head h / (n_q_heads / n_kv_heads);
  * a query that sees no key gets 0.  Keys and values a query does not see do not enter its result, whatever they hold.
  * Rows of q that belong to no sequence are not read, the same rows of out not written.  A sequence longer than
- * max_q_len / max_k_len or reaching beyond its arrays is skipped and flagged (RAG_FAULT_SEGMENT, RAG_FAULT_KV_ROW);
+ * max_q_len / max_k_len or reaching beyond its arrays is skipped and flagged (RAG_FAULT_SEGMENT, RAG_FAULT_KV_ROW; with max_q_len 0 nothing runs, nor is flagged);
  * without k_start, max_q_len stands for max_k_len, here and in the workspace's size.
- * dtype bf16, fp16 (matrix cores, fp32 softmax and sums) or fp32; head_dim 32, 64 or 128; pointers and strides multiples
+ * dtype bf16, fp16 or fp32.  Scores, softmax and sums are fp32; of the 16-bit types the softmax's weights are rounded to the type
+ * once before they meet the values (the sum they are divided by is of the unrounded ones), then the result is.  head_dim 32, 64 or 128; pointers and strides multiples
  * of 16 bytes, rows of k and v at most 32 MB apart; out must not overlap q, k or v.  workspace: rag_enc_attention_window_workspace() bytes for the same sizes (0:
  * may be NULL), 16-byte aligned, used by this call alone until it has run on its stream; what it holds before does not matter. */
 int64_t rag_enc_attention_window_workspace(int64_t total_q, int32_t n_seq, int32_t max_q_len, int32_t max_k_len,
@@ -595,10 +597,11 @@ int rag_enc_attention_window_dev(const void* d_q, int64_t q_stride, const void* 
 /* y[m][n] = sum_k x[m][k] w[n][k] + bias[n] with weights of 4 bits: w[n][k] = scales[n][k / group] * code + offsets[n][k / group],
  * without offsets (NULL) scales[n][k / group] * (code - 8).  codes [n][k / 2]: column 2i in the low half of byte i of
  * the row, column 2i + 1 in its high half; scales, offsets [n][k / group], bias [n] (or NULL) of x's type (bf16, fp16 or
- * fp32).  Made for the few rows of one query (the weights are read once per 16 or 32 rows of x).  fp32 sums.
+ * fp32).  Made for the few rows of one query (the weights are read once per 16 or 32 rows of x).  fp32 sums, of
+ * x times 16 + code, with the scales applied to the sums: about twice the error of fp32 sums of x times whole weights.
  * group 32, 64 or 128, k < 2^26 a multiple of it, n < 2^28, m up to 2 million; x, its rows and the codes aligned to 16 bytes, rows of
  * x at most 32 MB apart; y must not overlap x.  A row of x that holds an infinity or a NaN gives infinities or NaN;
- * finite rows give what fp32 sums of x times w give, also where sums of x and codes alone would overflow.         */
+ * finite rows give infinities or NaN only where fp32 sums of x times w do.                                        */
 int rag_enc_linear4_dev(const void* d_x, int64_t x_stride, const uint8_t* d_codes, const void* d_scales,
                         const void* d_offsets, const void* d_bias, int64_t m, int32_t n, int32_t k, int32_t group,
                         int32_t dtype, void* d_y, int64_t y_stride, void* stream);
