@@ -227,3 +227,30 @@ def test_float32_keeps_24_bits_of_x(m, n, k, group, offsets):
     err = rag_hip.enc_linear4_dev(x, codes, scales, off).double() - x.double() @ (c * s + o).t()
     square = x.double() ** 2 @ (((c + 16) * s) ** 2 + (o - 16 * s) ** 2).t()
     assert float(err.pow(2).mean().sqrt()) <= 8 * 2.0 ** -24 * float(square.mean().sqrt())
+
+
+@pytest.mark.parametrize('m', [1, 13])
+def test_weights_beyond_32_bits(m):
+    """The first and last rows of weights of more than 2^32 bytes."""
+    import rag_hip
+    n, k, group, part = (1 << 20) + 77, 8192, 128, 300
+    x, some, scales, off, bias = _operands(m, 2 * part, k, group, True, torch.bfloat16, m)
+    codes = torch.zeros((n, k // 2), dtype=torch.uint8, device=_dev())
+    s, o = (torch.zeros((n, k // group), dtype=torch.bfloat16, device=_dev()) for _ in range(2))
+    b = torch.zeros((n,), dtype=torch.bfloat16, device=_dev())
+    for to, at in ((slice(0, part), slice(0, part)), (slice(n - part, n), slice(part, 2 * part))):
+        codes[to], s[to], o[to], b[to] = some[at], scales[at], off[at], bias[at]
+    y = rag_hip.enc_linear4_dev(x, codes, s, o, b)
+    _check(torch.cat([y[:, :part], y[:, n - part:]], dim=1), x, some, scales, off, bias)
+    assert float(y[:, part:n - part].abs().max()) == 0.0
+
+
+def test_two_million_rows():
+    import rag_hip
+    m = 2097120                                                 # the most that a launch takes
+    x, codes, scales, off, bias = _operands(m, 3, 32, 32, True, torch.bfloat16, 2)
+    y = rag_hip.enc_linear4_dev(x, codes, scales, off, bias)
+    for part in (slice(0, 5000), slice(m - 5000, m)):
+        _check(y[part], x[part], codes, scales, off, bias)
+    with pytest.raises(rag_hip.RagHipError, match='too many rows'):
+        rag_hip.enc_linear4_dev(torch.cat([x, x[:1]]), codes, scales, off, bias)

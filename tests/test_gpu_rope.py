@@ -277,3 +277,21 @@ def test_an_infinity_under_the_norm(kind, inter):
     nan = torch.zeros((t, d), dtype=torch.bool, device=_dev())
     nan[0, 40] = nan[1, 3] = nan[1, 2 if inter else 3 + rot // 2] = True
     assert torch.equal(torch.isnan(q[:, 0]), nan) and float(q[:, 0][~nan].abs().max()) == 0.0
+
+
+def test_rows_beyond_32_bits():
+    """The first and last tokens of a projection of more than 2^32 elements."""
+    import rag_hip
+    t, d, n = (1 << 32) // 96 + 2000, 32, 1000
+    qkv = torch.zeros((t, 3 * d), dtype=torch.bfloat16, device=_dev())
+    for part in (slice(0, n), slice(t - n, t)):
+        qkv[part] = torch.randn((n, 3 * d), generator=_gen(4), device=_dev()).to(torch.bfloat16)
+    pos = torch.arange(t, dtype=torch.int32, device=_dev())
+    inv = rag_hip.rope_inv_freq(d)
+    q, k, v = _call(qkv, pos, inv, 1, 1, None, None, False)
+    for part in (slice(0, n), slice(t - n, t)):
+        x = qkv[part].view(n, 3, d)
+        _close(q[part], *_ref(x[:, :1], pos[part], inv, None, 1e-6, False))
+        _close(k[part], *_ref(x[:, 1:2], pos[part], inv, None, 1e-6, False))
+        assert torch.equal(v[part], x[:, 2:])
+    assert float(q[n:t - n].abs().max()) == 0.0

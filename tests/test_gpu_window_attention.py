@@ -594,3 +594,54 @@ def test_values_near_the_end_of_the_range(kind, hq, hkv, d, q_lens, k_lens, left
     got = rag_hip.enc_attention_window_dev(q, k, v, _cu(q_lens), max(q_lens), window_left=left, window_right=right, **kw)
     assert bool(torch.isfinite(got).all())
     _check(got, q, k, v, q_lens, list(zip(_cu(k_rows).tolist(), k_rows)), left, right, 0, d ** -0.5)
+
+
+@pytest.mark.parametrize('nq,nk', [(3, 900), (1, 20000), (300, 400), (60, 3000)])
+def test_queries_beyond_32_bits(nq, nk):
+    """The last rows of queries of more than 2^32 elements; the rows in front of them belong to no sequence."""
+    import rag_hip
+    hq, hkv, d, g = 32, 8, 128, _gen(nq)
+    rows = (1 << 32) // (hq * d) + 1000
+    q = torch.zeros((rows, hq, d), dtype=torch.bfloat16, device=_dev())
+    q[-nq:] = torch.randn((nq, hq, d), generator=g, device=_dev()).to(torch.bfloat16)
+    k, v = (torch.randn((nk, hkv, d), generator=g, device=_dev()).to(torch.bfloat16) for _ in range(2))
+    out = torch.full((rows, hq * d), 7.0, dtype=torch.bfloat16, device=_dev())
+    rag_hip.enc_attention_window_dev(q, k, v, torch.tensor([rows - nq, rows], dtype=torch.int32, device=_dev()), nq, k_start=torch.zeros(1, dtype=torch.int64, device=_dev()),
+                                     k_len=torch.tensor([nk], dtype=torch.int32, device=_dev()), max_k_len=nk, window_right=0, out=out)
+    _check(out[-nq:], q[-nq:], k, v, [nq], [(0, nk)], -1, 0, 0, d ** -0.5)
+    assert bool((out[:-nq] == 7).all())
+
+
+@pytest.mark.parametrize('nq,nk', [(1, 5000), (200, 200), (60, 3000)])
+def test_windows_beyond_every_length_are_no_windows(nq, nk):
+    import rag_hip
+    g, far = _gen(8), (1 << 31) - 1
+    q = torch.randn((nq, 4, 64), generator=g, device=_dev()).to(torch.float16)
+    k, v = (torch.randn((nk, 2, 64), generator=g, device=_dev()).to(torch.float16) for _ in range(2))
+    kw = dict(k_start=torch.zeros(1, dtype=torch.int64, device=_dev()), k_len=torch.tensor([nk], dtype=torch.int32, device=_dev()), max_k_len=nk)
+    want = rag_hip.enc_attention_window_dev(q, k, v, _cu([nq]), nq, **kw)
+    for left, right, sinks in ((far, far, 0), (far, -1, far), (-1, 1 << 30, 5), (1 << 30, far, 0)):
+        assert torch.equal(want, rag_hip.enc_attention_window_dev(q, k, v, _cu([nq]), nq, window_left=left, window_right=right, n_sinks=sinks, **kw))
+    near = (1 << 30) - 1                                        # the longest that is one: every key in it, by another path perhaps
+    got = rag_hip.enc_attention_window_dev(q, k, v, _cu([nq]), nq, window_left=near, window_right=near, n_sinks=far, **kw)
+    _check(got, q, k, v, [nq], [(0, nk)], -1, -1, 0, 0.125)
+
+
+@pytest.mark.parametrize('kind', list(TYPES))
+@pytest.mark.parametrize('nq,nk', [(3, 40), (4, 5000), (200, 200), (60, 3000)])
+def test_a_query_that_is_not_finite_spoils_its_own_row_only(kind, nq, nk):
+    import rag_hip
+    dt, g = TYPES[kind], _gen(nq)
+    q = torch.randn((nq, 4, 64), generator=g, device=_dev()).to(dt)
+    k, v = (torch.randn((nk, 2, 64), generator=g, device=_dev()).to(dt) for _ in range(2))
+    bad = q.clone()
+    bad[1, 2, 5], bad[2, 0, 7], bad[0, 3, 63] = float('nan'), float('inf'), -float('inf')
+    got = rag_hip.enc_attention_window_dev(bad, k, v, _cu([nq]), nq, k_start=torch.zeros(1, dtype=torch.int64, device=_dev()),
+                                           k_len=torch.tensor([nk], dtype=torch.int32, device=_dev()), max_k_len=nk, window_right=0).view(nq, 4, 64)
+    assert bool(torch.isnan(got[1, 2]).all())
+    ref = rag_hip.enc_attention_window_dev(q, k, v, _cu([nq]), nq, k_start=torch.zeros(1, dtype=torch.int64, device=_dev()),
+                                           k_len=torch.tensor([nk], dtype=torch.int32, device=_dev()), max_k_len=nk, window_right=0).view(nq, 4, 64).clone()
+    rest = torch.ones((nq, 4), dtype=torch.bool, device=_dev())
+    rest[1, 2] = rest[2, 0] = rest[0, 3] = False
+    mixed = torch.where(rest[:, :, None], got, ref)
+    _check(mixed.reshape(nq, -1), q, k, v, [nq], [(0, nk)], -1, 0, 0, 0.125)
