@@ -232,7 +232,8 @@ constexpr float LAG = 8.f;           // the maximum may lag behind by this power
 //   O^T += V^T P^T     the lane's probabilities are the B operand as they stand; V^T comes out of the row-major image
 //                      through the transposing LDS read
 // 16-bit types: probabilities are rounded to the type (half a step of each; the result is as far from the exact one again as
-// its own rounding takes it), their sum and all other sums are fp32.
+// its own rounding takes it), their sum and all other sums are fp32.  In two parts they would cost a second product with the
+// values and as much again to cut: 16384 tokens, window 4096, 485 -> 658 us, passages of up to 512 tokens 34.7 -> 40.3.
 // fp32: queries, keys, values and probabilities as sums of three bf16 each, exactly; of the nine products the six that reach
 // 2^-20 of the factors are taken (the other three stay below 2^-20 together, an fp32 sum over 32 dimensions may be off by 2^-19), all in fp32.
 // The matrix cores do six bf16 products in 3/8 of the time of an fp32 one: 4096 tokens, causal, 16 heads of 128 on 8: 411 us,
@@ -598,8 +599,10 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 // products, 16 * QT of them per workgroup, so that a key is read once for all of them.  Its waves take tiles of keys in
 // turn, each into its own two LDS buffers (no barrier until the end), and put their results together; a long text is cut
 // into spans of `span` tiles, one workgroup each, whose results the last of them puts together, or window_join_kernel.
-// Probabilities are rounded to a 16-bit type as above (float32 takes fp32 products, in which nothing is rounded); 64 rows of
-// float32 at head size 128 are more than the registers hold (44 go to scratch).
+// Probabilities of a 16-bit type: up to 16 rows they are taken in two parts, at 16 bits or more, which costs 0 to 2 % there (one token over
+// a window of 1024 8.4 and 8.5 us, 16 tokens on 4000 to 32768 keys 188.8 both); beyond, rounded to the type as above (7 % for 64
+// rows).  float32 takes fp32 products, in which nothing is rounded; 64 rows of it at head size 128 are more than the registers
+// hold (44 go to scratch).
 // Bound by the bytes of the keys and values, 64 KB of them in flight per compute unit at head size 128: 16 tokens over 4000 to
 // 32768 kept rows of 8 heads in 0.19 ms, 5.1 TB/s (a large copy moves 4.7).  One token over a window of 1024: 8.4 us, of which the
 // launch, the loads of the arguments and the queries, and joining the spans are three quarters.
@@ -860,11 +863,16 @@ __global__ __launch_bounds__(64 * (FewImage<E, D>::NW), (FewImage<E, D>::waves(1
             }
         } else {
             typedef short tr4 __attribute__((__vector_size__(4 * sizeof(short))));
-            typename Mma<E>::x8 pb[QT];
+            constexpr bool TWO = QT == 1;                     // probabilities as the type's value and what it leaves
+            typename Mma<E>::x8 pb[QT], rest[QT];
 #pragma unroll
             for (int qt = 0; qt < QT; ++qt)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) pb[qt][j] = (E)s[qt][(j >> 2) % KB][j & 3];
+                for (int j = 0; j < 8; ++j) {
+                    const float p = s[qt][(j >> 2) % KB][j & 3];
+                    pb[qt][j] = (E)p;
+                    if (TWO) rest[qt][j] = (E)(p - (float)pb[qt][j]);
+                }
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
                 union { tr4 t[2]; typename Mma<E>::x8 v; } av;
@@ -875,7 +883,10 @@ __global__ __launch_bounds__(64 * (FewImage<E, D>::NW), (FewImage<E, D>::waves(1
                     av.t[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) tr4*)p);
                 }
 #pragma unroll
-                for (int qt = 0; qt < QT; ++qt) o[qt][dt] = MmaFew<E>::mfma(av.v, pb[qt], o[qt][dt]);
+                for (int qt = 0; qt < QT; ++qt) {
+                    if (TWO) o[qt][dt] = MmaFew<E>::mfma(av.v, rest[qt], o[qt][dt]);
+                    o[qt][dt] = MmaFew<E>::mfma(av.v, pb[qt], o[qt][dt]);
+                }
             }
         }
     }

@@ -581,7 +581,8 @@ int rag_enc_qk_norm_rope_dev(const void* d_qkv, int64_t qkv_stride, const int32_
  * max_q_len / max_k_len or reaching beyond its arrays is skipped and flagged (RAG_FAULT_SEGMENT, RAG_FAULT_KV_ROW; with max_q_len 0 nothing runs, nor is flagged);
  * without k_start, max_q_len stands for max_k_len, here and in the workspace's size.
  * dtype bf16, fp16 or fp32.  Scores, softmax and sums are fp32; of the 16-bit types the softmax's weights are rounded to the type
- * once before they meet the values (the sum they are divided by is of the unrounded ones), then the result is.  head_dim 32, 64 or 128; pointers and strides multiples
+ * once before they meet the values (the sum they are divided by is of the unrounded ones; not in calls of at most 16 rows, max_q_len
+ * times the query heads of a key/value head, that the few-query kernel takes), then the result is.  head_dim 32, 64 or 128; pointers and strides multiples
  * of 16 bytes, rows of k and v at most 32 MB apart; out must not overlap q, k or v.  workspace: rag_enc_attention_window_workspace() bytes for the same sizes (0:
  * may be NULL), 16-byte aligned, used by this call alone until it has run on its stream; what it holds before does not matter. */
 int64_t rag_enc_attention_window_workspace(int64_t total_q, int32_t n_seq, int32_t max_q_len, int32_t max_k_len,
