@@ -122,7 +122,7 @@ __device__ void attend_row(const WinArgs& a, const Seq& sq, int j, int head, int
     for (int o = DL; o < 64; o <<= 1) { o0 += __shfl_xor(o0, o, 64); o1 += __shfl_xor(o1, o, 64); }
     if (part == 0) {
         T* dst = reinterpret_cast<T*>(a.out) + (sq.q0 + j) * a.out_stride + (int64_t)head * D + d0;
-        dst[0] = (T)(total == 0 ? 0.f : l > 0.f ? o0 : NAN);  // (l: 0 where every score is -infinity, NaN where one is)
+        dst[0] = (T)(total == 0 ? 0.f : l > 0.f ? o0 : NAN);  // (l: 0 where every score is -infinity, NaN where one is NaN)
         dst[1] = (T)(total == 0 ? 0.f : l > 0.f ? o1 : NAN);
     }
 }
